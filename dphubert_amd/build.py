@@ -17,19 +17,30 @@ LIB = HERE / "libdphubert_hip.so"
 OBJ = HERE / "csrc" / "build"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
-FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I", str(INCLUDE), "-Wno-unused-result"]
+# packed fp32 instructions are off: some of their forms have given wrong results on this hardware
+FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I", str(INCLUDE), "-Wno-unused-result",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _sources():
     return sorted(CSRC.glob("*.hip"))
 
 
+def _deps(src: Path, obj: Path):
+    """The source and this tree's headers that its last compilation read (all of them if that is not known)."""
+    deps = [src] + list(CSRC.glob("*.h")) + list(INCLUDE.glob("*.h"))
+    dfile = obj.with_suffix(".d")
+    if dfile.exists():
+        read = {Path(p).resolve() for p in dfile.read_text().replace("\\\n", " ").split()[1:]}
+        deps = [src] + [h for h in deps[1:] if h.resolve() in read]
+    return deps
+
+
 def _compile(src: Path) -> Path:
     obj = OBJ / (src.stem + ".o")
-    deps = [src] + list(CSRC.glob("*.h")) + list(INCLUDE.glob("*.h"))
-    if obj.exists() and obj.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
+    if obj.exists() and obj.stat().st_mtime >= max(d.stat().st_mtime for d in _deps(src, obj)):
         return obj
-    cmd = [HIPCC] + FLAGS + ["-c", str(src), "-o", str(obj)]
+    cmd = [HIPCC] + FLAGS + ["-MD", "-MF", str(obj.with_suffix(".d")), "-c", str(src), "-o", str(obj)]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src.name}:\n{r.stderr[-6000:]}")
@@ -39,11 +50,16 @@ def _compile(src: Path) -> Path:
 def build(force: bool = False, jobs: int = 8) -> Path:
     OBJ.mkdir(parents=True, exist_ok=True)
     srcs = _sources()
+    # objects of other flags are stale too
+    stamp = OBJ / "flags"
+    if not stamp.exists() or stamp.read_text() != " ".join(FLAGS):
+        force = True
     if force:
         for o in OBJ.glob("*.o"):
             o.unlink()
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
         objs = list(ex.map(_compile, srcs))
+    stamp.write_text(" ".join(FLAGS))
     if LIB.exists() and not force and LIB.stat().st_mtime >= max(o.stat().st_mtime for o in objs):
         return LIB
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(LIB)] + [str(o) for o in objs]
