@@ -64,6 +64,25 @@ class DphHcEntry(C.Structure):
     _fields_ = [("log_alpha", vp), ("u_in", vp), ("dmask", vp), ("dlog_alpha", vp), ("n", i64), ("offset", i64)]
 
 
+class DphLinearI8Args(C.Structure):
+    _fields_ = [("M", i64), ("N", i64), ("K", i64), ("x", vp), ("ldx", i64), ("x_f32", i32), ("act", i32),
+                ("ln_weight", vp), ("ln_bias", vp), ("norm_out", vp), ("ld_norm", i64), ("q", vp), ("ldq", i64),
+                ("q_scale", vp), ("w", vp), ("ldw", i64), ("w_scale", vp), ("bias", vp), ("residual", vp), ("ldr", i64),
+                ("out", vp), ("ldo", i64), ("residual_f32", i32), ("out_dtype", i32), ("ln_eps", f32),
+                ("reserved", i32)]
+
+
+class DphNsMat(C.Structure):
+    _fields_ = [("p", vp), ("row_stride", i64), ("col_stride", i64)]
+
+
+class DphNsGroup(C.Structure):
+    _fields_ = [("rows", i64), ("cols", i64), ("count", i64), ("out", vp), ("f32", i32), ("reserved", i32)]
+
+
+I8_K_MAX = 131072
+I8_LN_MAX = 2048
+
 S = vp  # hipStream_t
 
 _SIGS = {
@@ -167,6 +186,11 @@ _SIGS = {
     "dph_adamw_step": ([vp, i64, vp, vp, i64, vp, i64, i64, vp, f32, S], C.c_int),
     "dph_adamw_step_dev": ([vp, i64, vp, vp, i64, vp, vp, f32, S], C.c_int),
     "dph_adamw_step_img": ([vp, i64, vp, vp, i64, vp, vp, i64, i64, vp, f32, vp, S], C.c_int),
+    "dph_quant_rows_i8": ([vp, C.c_int, i64, i64, i64, vp, i64, vp, S], C.c_int),
+    "dph_linear_i8": ([C.POINTER(DphLinearI8Args), S], C.c_int),
+    "dph_newton_schulz_workspace": ([C.POINTER(DphNsGroup), i64], i64),
+    "dph_newton_schulz": ([C.POINTER(DphNsMat), C.POINTER(DphNsGroup), i64, i64, C.POINTER(f32), f32, vp, i64, S],
+                          C.c_int),
     "dph_set_rng_epoch": ([vp], C.c_int),
     "dph_event_create": ([C.POINTER(vp)], C.c_int),
     "dph_event_record": ([vp, S], C.c_int),
@@ -185,8 +209,9 @@ _lib = None
 # 23: dph_discard_reductions / dph_reductions_pushed, queue-flush launch errors propagated by every column reduction;
 #     DphGemmArgs.sk_* + dph_gemm_sk_plan: the persistent stream-K 256 x 256 GEMM;
 # 24: dph_attention_bwd_qv / dph_attention_bwd_relpos_qv + dph_attention_bwd_qv_workspace: the q / v bias
-#     gradients summed inside the attention backward)
-ABI_VERSION = 24
+#     gradients summed inside the attention backward;
+# 25: dph_quant_rows_i8 / dph_linear_i8: 8-bit integer products; dph_newton_schulz)
+ABI_VERSION = 25
 
 
 class DphError(RuntimeError):

@@ -8,7 +8,7 @@ inside the library.
 
 import ctypes as C
 import os
-from typing import Optional, Sequence
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -463,3 +463,248 @@ def linear_wgrad_grouped(items: Sequence, accumulate: bool = True) -> Optional[t
             name = f"{name} grouped M={N} N={K} K={M} b={n} s={splits}"
         prof.records.append((name, 2.0 * M * N * K * n, e0, e1, n * (2.0 * (M * N + M * K) + 8.0 * N * K), ROLE[0]))
     return ws
+
+
+# ---------------------------------------------------------------------------
+# 8-bit integer products (int8.hip) and Newton-Schulz orthogonalisation (newton_schulz.hip)
+# ---------------------------------------------------------------------------
+class I8Rows(NamedTuple):
+    """Rows as 8-bit integers with one fp32 scale each: row r stands for ``q[r] * scale[r]``.  ``q`` is [R, K] int8 with
+    rows that start a multiple of 16 bytes apart, as quant_rows_i8 makes them."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+class _on_device:
+    """The tensors' device is the current one inside the block (and torch's current stream of it the launch stream)."""
+
+    def __init__(self, dev):
+        self.guard = torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _chk_on(dev, t, name, dtypes, ndim):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor (no CPU path)")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the input on {dev}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    if t.dim() != ndim:
+        raise ValueError(f"{name}: expected {ndim} dimensions, got shape {tuple(t.shape)}")
+
+
+def _chk_rows(t, name):
+    """[R, K] rows of unit stride that do not overlap; their distance in elements."""
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous (strides {t.stride()})")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}: rows overlap (strides {t.stride()})")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _chk_i8(dev, r, name):
+    """The distance of the rows of an I8Rows in bytes."""
+    _chk_on(dev, r.q, name + ".q", (torch.int8,), 2)
+    _chk_on(dev, r.scale, name + ".scale", (F32,), 1)
+    if r.scale.shape[0] != r.q.shape[0] or not r.scale.is_contiguous():
+        raise ValueError(f"{name}: {r.q.shape[0]} rows and a scale of shape {tuple(r.scale.shape)}, "
+                         f"strides {r.scale.stride()}")
+    R, K = r.q.shape
+    ld = _chk_rows(r.q, name + ".q")
+    if R == 1:
+        ld = (ld + 15) // 16 * 16
+    ends = r.q.storage_offset() + (R - 1) * ld + (K + 15) // 16 * 16
+    if R and (ld % 16 or r.q.data_ptr() % 16 or ends > r.q.untyped_storage().nbytes()):
+        raise ValueError(f"{name}.q: rows must start (and be readable to) a multiple of 16 bytes, as quant_rows_i8 lays "
+                         f"them out; shape {tuple(r.q.shape)}, strides {r.q.stride()}")
+    return ld
+
+
+def _i8_ld(K: int) -> int:
+    return (K + 15) // 16 * 16
+
+
+def quant_rows_i8(x: torch.Tensor) -> I8Rows:
+    """x [R, K] bf16 / fp32 -> 8-bit integers with one scale a row (a token of activations, an output channel of an
+    nn.Linear weight): ``scale = max|x| * (1 / 127)`` in fp32 (at least 2^-126), ``q = x / scale`` to the nearest integer, ties to
+    even.  A row with an infinity or a NaN has the scale NaN: all that is computed from it is NaN.  Rows of x may lie
+    apart (row-strided views)."""
+    if not isinstance(x, torch.Tensor):
+        raise ValueError("x must be a device tensor (no CPU path)")
+    _chk_on(x.device, x, "x", (BF16, F32), 2)
+    R, K = x.shape
+    if not 1 <= K <= _lib.I8_K_MAX:
+        raise ValueError(f"x: rows of 1 to {_lib.I8_K_MAX} elements, got {K}")
+    ldx = _chk_rows(x, "x")
+    ld = _i8_ld(K)
+    with _on_device(x.device):
+        q = torch.empty(R, ld, dtype=torch.int8, device=x.device)
+        scale = torch.empty(R, dtype=F32, device=x.device)
+        if R:
+            call("dph_quant_rows_i8", ptr(x), int(x.dtype == F32), R, K, ldx, ptr(q), ld, ptr(scale), _stream())
+    return I8Rows(q[:, :K] if ld != K else q, scale)
+
+
+def _linear_i8(x, w, bias, act, residual, out, out_dtype, ln, keep_norm):
+    rows = isinstance(x, I8Rows)
+    t = x.q if rows else x
+    if not isinstance(t, torch.Tensor):
+        raise ValueError("x must be a device tensor (no CPU path)")
+    dev = t.device
+    if rows:
+        ldq = _chk_i8(dev, x, "x")
+    else:
+        _chk_on(dev, x, "x", (BF16, F32), 2)
+    if not isinstance(w, I8Rows):
+        raise ValueError("w must be an I8Rows (quant_rows_i8 of the nn.Linear weight)")
+    ldw = _chk_i8(dev, w, "w")
+    M, K = t.shape
+    N = w.q.shape[0]
+    if w.q.shape[1] != K:
+        raise ValueError(f"x has rows of {K} elements, w of {w.q.shape[1]}")
+    if not 1 <= K <= _lib.I8_K_MAX:
+        raise ValueError(f"x: rows of 1 to {_lib.I8_K_MAX} elements, got {K}")
+    if act not in (ACT_NONE, ACT_GELU):
+        raise ValueError(f"act must be ACT_NONE or ACT_GELU, got {act}")
+    a = _lib.DphLinearI8Args()
+    if bias is not None:
+        _chk_on(dev, bias, "bias", (F32,), 1)
+        if bias.shape[0] != N or not bias.is_contiguous():
+            raise ValueError(f"bias: expected {N} contiguous elements, got shape {tuple(bias.shape)}")
+        a.bias = ptr(bias)
+    if residual is not None:
+        _chk_on(dev, residual, "residual", (BF16, F32), 2)
+        if tuple(residual.shape) != (M, N):
+            raise ValueError(f"residual: expected {(M, N)}, got {tuple(residual.shape)}")
+        out_dtype = residual.dtype
+        a.ldr = _chk_rows(residual, "residual")
+        a.residual, a.residual_f32 = ptr(residual), int(out_dtype == F32)
+    if out_dtype not in (BF16, F32):
+        raise ValueError(f"out_dtype must be bf16 or fp32, got {out_dtype}")
+    norm = None
+    with _on_device(dev):
+        if out is None:
+            out = torch.empty(M, N, dtype=out_dtype, device=dev)
+        else:
+            _chk_on(dev, out, "out", (out_dtype,), 2)
+            if tuple(out.shape) != (M, N):
+                raise ValueError(f"out: expected {(M, N)}, got {tuple(out.shape)}")
+        a.ldo = _chk_rows(out, "out")
+        a.M, a.N, a.K, a.act = M, N, K, act
+        if not rows:
+            a.x, a.x_f32, a.ldx = ptr(x), int(x.dtype == F32), _chk_rows(x, "x")
+            ldq = _i8_ld(K)
+            ws = torch.empty(M * (ldq + 4), dtype=torch.int8, device=dev)    # q, then the scales
+            a.q, a.q_scale = ws.data_ptr(), ws.data_ptr() + M * ldq
+            if ln is not None:
+                a.ln_weight, a.ln_bias, a.ln_eps = ptr(ln[0]), ptr(ln[1]), ln[2]
+                if keep_norm:
+                    norm = torch.empty(M, K, dtype=BF16, device=dev)
+                    a.norm_out, a.ld_norm = ptr(norm), K
+        else:
+            a.q, a.q_scale = ptr(x.q), ptr(x.scale)
+        a.ldq = ldq
+        a.w, a.ldw, a.w_scale = ptr(w.q), ldw, ptr(w.scale)
+        a.out, a.out_dtype = ptr(out), OUT_F32 if out_dtype == F32 else OUT_BF16
+        if M:
+            call("dph_linear_i8", C.byref(a), _stream())
+    return out, norm
+
+
+def linear_i8(x: Union[torch.Tensor, I8Rows], w: I8Rows, bias: Optional[torch.Tensor] = None, *, act: int = ACT_NONE,
+              residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+              out_dtype: torch.dtype = BF16) -> torch.Tensor:
+    """y = act(x W^T + bias) + residual in 8-bit integers (forward only: inference, a frozen teacher).
+
+    x [M, K] bf16 / fp32 (quantised here, one scale a token) or the I8Rows of it; w: quant_rows_i8 of the nn.Linear
+    weight [N, K]; bias [N] fp32; act ACT_NONE / ACT_GELU; residual [M, N] bf16 / fp32, whose type the output takes
+    (without one ``out_dtype``).  Integer sums are exact; scales, bias, activation and residual are applied in fp32.
+    K up to 131072.  x, residual and out may be row-strided; out may be the residual itself."""
+    return _linear_i8(x, w, bias, act, residual, out, out_dtype, None, False)[0]
+
+
+def layernorm_linear_i8(x: torch.Tensor, ln_weight: torch.Tensor, ln_bias: torch.Tensor, w: I8Rows,
+                        bias: Optional[torch.Tensor] = None, *, act: int = ACT_NONE, eps: float = 1e-5,
+                        keep_norm: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(linear_i8 of LayerNorm(x), the LayerNorm's output in bf16 where ``keep_norm``, else None).
+
+    x [M, K] bf16 / fp32, K up to 2048; statistics, the normalised values and the tokens' scales are fp32: the integers
+    come from the values before their rounding to bf16.  The product is bf16."""
+    if not isinstance(x, torch.Tensor):
+        raise ValueError("x must be a device tensor (no CPU path)")
+    _chk_on(x.device, x, "x", (BF16, F32), 2)
+    K = x.shape[1]
+    if not 1 <= K <= _lib.I8_LN_MAX:
+        raise ValueError(f"x: rows of 1 to {_lib.I8_LN_MAX} elements, got {K}")
+    for t, name in ((ln_weight, "ln_weight"), (ln_bias, "ln_bias")):
+        _chk_on(x.device, t, name, (F32,), 1)
+        if t.shape[0] != K or not t.is_contiguous():
+            raise ValueError(f"{name}: expected {K} contiguous elements, got shape {tuple(t.shape)}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    return _linear_i8(x, w, bias, act, None, None, BF16, (ln_weight, ln_bias, float(eps)), keep_norm)
+
+
+NS_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def newton_schulz(mats: Sequence[torch.Tensor], *, steps: int = 5, coeffs: Sequence[float] = NS_COEFFS,
+                  eps: float = 1e-7) -> List[torch.Tensor]:
+    """The orthogonal factor of every matrix of the list, approximately: ``steps`` quintic Newton-Schulz steps
+    X <- a X + (b A + c A^2) X, A = X X^T, from X = G / (|G|_F + eps) (of G^T where G is taller than wide).
+
+    mats: 2-D tensors of one device, bf16 or fp32, of any shapes and row strides (a transposed view will do).  Returns
+    bf16 tensors of the same shapes.  Matrices of one shape share launches, so hand in a whole model's at once.  The
+    results are within about two bf16 roundings of the iteration in 64 bits (newton_schulz.hip)."""
+    mats = list(mats)
+    if not mats:
+        return []
+    dev = mats[0].device if isinstance(mats[0], torch.Tensor) else None
+    if not 1 <= int(steps) <= 64:
+        raise ValueError(f"steps must be 1 to 64, got {steps}")
+    if len(coeffs) != 3:
+        raise ValueError(f"coeffs are (a, b, c), got {coeffs}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    places = {}
+    for i, t in enumerate(mats):
+        _chk_on(dev, t, f"mats[{i}]", (BF16, F32), 2)
+        R, K = t.shape
+        if not (R and K):
+            raise ValueError(f"mats[{i}] is empty: {tuple(t.shape)}")
+        s0, s1 = t.stride()
+        if not ((s1 == 1 or K == 1) and (s0 >= K or R == 1)) and not ((s0 == 1 or R == 1) and (s1 >= R or K == 1)):
+            raise ValueError(f"mats[{i}]: rows or columns must be contiguous and apart, strides {t.stride()}")
+        places.setdefault((R, K, t.dtype), []).append(i)
+    arr = (_lib.DphNsMat * len(mats))()
+    grp = (_lib.DphNsGroup * len(places))()
+    out = [None] * len(mats)
+    with _on_device(dev):
+        k = 0
+        for gi, ((R, K, dt), at) in enumerate(places.items()):
+            res = torch.empty(len(at), R, K, dtype=BF16, device=dev)
+            grp[gi].rows, grp[gi].cols, grp[gi].count = R, K, len(at)
+            grp[gi].out, grp[gi].f32 = res.data_ptr(), int(dt == F32)
+            for i, o in zip(at, res.unbind()):
+                out[i] = o
+                s0, s1 = mats[i].stride()
+                by_row = (s1 == 1 or K == 1) and (s0 >= K or R == 1)
+                arr[k].p = mats[i].data_ptr()
+                # (the stride of a dimension of one element is whatever the view says: it is never used)
+                arr[k].row_stride, arr[k].col_stride = (max(s0, K), 1) if by_row else (1, max(s1, R))
+                k += 1
+        nbytes = _lib.lib().dph_newton_schulz_workspace(grp, len(places))
+        if nbytes < 0:
+            _lib.check(-1, "dph_newton_schulz_workspace")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        call("dph_newton_schulz", arr, grp, len(places), int(steps), (C.c_float * 3)(*coeffs), float(eps), ptr(ws),
+             nbytes, _stream())
+    return out

@@ -635,6 +635,71 @@ int dph_event_record(void* ev, hipStream_t stream);
 int dph_event_elapsed_ms(void* start, void* stop, float* ms);
 int dph_event_destroy(void* ev);
 
+/* ---- 8-bit integer products (ABI 25) ------------------------------------------------------------------------------
+ * Rows as 8-bit integers with one fp32 scale each: scale = max(max |x| * (1.0f / 127.0f), 2^-126), q = x / scale to the nearest
+ * integer of the exact quotient, ties to even.  A row that holds an infinity or a NaN has the scale NaN and q = 0, so
+ * whatever is computed from it is NaN and other rows are not touched.
+ * dph_quant_rows_i8: x [rows][K] bf16 (x_f32 != 0: fp32), rows ldx elements apart; q rows ldq bytes apart (a multiple
+ * of 16, at least K; the bytes from K to ldq are written as zeros), scale [rows]. */
+#define DPH_I8_K_MAX 131072   /* 127^2 K fits the 32-bit sums */
+#define DPH_I8_LN_MAX 2048
+int dph_quant_rows_i8(const void* x, int x_f32, int64_t rows, int64_t K, int64_t ldx, int8_t* q, int64_t ldq,
+                      float* scale, hipStream_t stream);
+
+/* y[m][n] = act( q_scale[m] w_scale[n] sum_k q[m][k] w[n][k] + bias[n] ) + residual[m][n]  (nn.Linear's forward with an
+ * activation and a residual, components.py:376-385, 715-748, on integers).
+ * x NULL: q / q_scale are given.  Otherwise x [M][K] is quantised into them first (dph_quant_rows_i8), and with
+ * ln_weight / ln_bias [K] its LayerNorm (K up to DPH_I8_LN_MAX) is, from the fp32 values; norm_out then receives these
+ * in bf16 (NULL: not).  w rows ldw bytes apart (a multiple of 16), bias may be NULL.  act: DPH_ACT_NONE / _GELU.
+ * residual (NULL: none) has out's type.  The sums are 32-bit integers, everything after them fp32.  What stands between
+ * K and the end of a row of q or w has no effect (it is read up to the next 16 bytes).  out must not overlap an input
+ * other than the residual it replaces element for element. */
+typedef struct DphLinearI8Args {
+  int64_t M, N, K;
+  const void* x;
+  int64_t ldx;
+  int32_t x_f32, act;
+  const float* ln_weight;
+  const float* ln_bias;
+  void* norm_out;
+  int64_t ld_norm;
+  int8_t* q;
+  int64_t ldq;
+  float* q_scale;
+  const int8_t* w;
+  int64_t ldw;
+  const float* w_scale;
+  const float* bias;
+  const void* residual;
+  int64_t ldr;
+  void* out;
+  int64_t ldo;
+  int32_t residual_f32, out_dtype; /* DPH_OUT_BF16 / DPH_OUT_F32 */
+  float ln_eps;
+  int32_t reserved;
+} DphLinearI8Args;
+int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream);
+
+/* ---- Newton-Schulz orthogonalisation (ABI 25) ---------------------------------------------------------------------
+ * For every matrix G [rows][cols] of the groups (one shape and type each): X0 = G / (|G|_F + eps) (the smaller side
+ * first), `steps` times X <- a X + (b A + c A^2) X with A = X X^T and coeffs = {a, b, c}, the result in bf16 to the
+ * group's out [count][rows][cols] (dense, 8-byte aligned).  mats: the groups' matrices one after the other; one of a
+ * matrix's strides is 1.  Operands are fp16, sums fp32 (newton_schulz.hip).  The result does not depend on the other
+ * matrices of the list.  A zero matrix gives zeros, one with an infinity or a NaN gives NaN throughout. */
+#define DPH_NS_MAX 1048576
+typedef struct DphNsMat {
+  const void* p;
+  int64_t row_stride, col_stride;
+} DphNsMat;
+typedef struct DphNsGroup {
+  int64_t rows, cols, count;
+  void* out;
+  int32_t f32, reserved; /* matrices are fp32 (else bf16) */
+} DphNsGroup;
+int64_t dph_newton_schulz_workspace(const DphNsGroup* groups, int64_t n_groups); /* bytes; -1: refused */
+int dph_newton_schulz(const DphNsMat* mats, const DphNsGroup* groups, int64_t n_groups, int64_t steps,
+                      const float* coeffs, float eps, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
