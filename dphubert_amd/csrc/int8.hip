@@ -6,6 +6,8 @@
 // quantised on the way in, a row at a time, either as they stand or as the output of a LayerNorm.
 #include "mfma_tile.h"
 
+#include <stdlib.h>
+
 #include <type_traits>
 
 namespace dph {
@@ -255,14 +257,16 @@ __device__ __forceinline__ void store_tile(const LinearI8& a, const mt::i32x4_t 
 }
 
 template <class C, bool GELU, int RES, bool OUT32>
-__global__ void __launch_bounds__(C::NT, 2) linear_i8_kernel(const LinearI8 a) {
-  __shared__ __align__(16) char smem[C::LDS];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int t = mt::xcd_tile((int)blockIdx.x, a.ntiles);
-  const int m0 = t / a.ntn * C::BM, n0 = t % a.ntn * C::BN;
+__global__ void __launch_bounds__(C::NT, C::WPE) linear_i8_kernel(const LinearI8 a) {
+  __shared__ __align__(1024) char smem[C::LDS];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  // tiles of one XCD: GM rows of tiles, column by column, so that its L2 holds both operands of what runs there
+  constexpr int GM = C::BM > 128 ? 4 : 8;
+  const int t = mt::xcd_tile((int)blockIdx.x, a.ntiles), per = GM * a.ntn, ntm = a.ntiles / a.ntn;
+  const int first = t / per * GM, h = min(GM, ntm - first), l = t % per;
+  const int m0 = (first + l % h) * C::BM, n0 = l / h * C::BN;
   mt::i32x4_t acc[C::FM][C::FN];
-  mt::clear<mt::I8, C>(acc);
-  mt::product<mt::I8, C>(a.x, a.w, a.K, m0, n0, acc, smem, wave, lane);
+  mt::product_of<mt::I8, C>(a.x, a.w, a.K, m0, n0, acc, smem, wave, lane, [&]() { mt::clear<mt::I8, C>(acc); });
   store_tile<C, GELU, RES, OUT32>(a, acc, m0 + wave / C::WC * C::WTM, n0 + wave % C::WC * C::WTN, lane);
 }
 
@@ -369,16 +373,32 @@ extern "C" int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream) {
   DPH_REQUIRE(a.ldw >= a.K && a.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0,
               "dph_linear_i8: rows of w start 16 bytes apart or a multiple of it");
   DPH_REQUIRE(a.ldo >= a.N || a.M == 1, "dph_linear_i8: rows of out overlap");
-  using C = mt::Tile<128, 128, 2, 2>;
-  const int64_t ntm = cdiv(a.M, C::BM), ntn = cdiv(a.N, C::BN);
-  DPH_REQUIRE(ntm * ntn < (1 << 23), "dph_linear_i8: too many tiles");
+  DPH_REQUIRE(a.ldq < (1 << 23) && a.ldw < (1 << 23), "dph_linear_i8: rows of q and w less than 2^23 bytes apart");
   const int es = out32 ? 4 : 2;
   const uintptr_t al = reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.residual) |
                        (uintptr_t)(a.ldo * es) | (uintptr_t)(a.residual ? a.ldr * es : 0);
   LinearI8 p{{reinterpret_cast<const char*>(a.q), a.ldq, (int32_t)a.M},
              {reinterpret_cast<const char*>(a.w), a.ldw, (int32_t)a.N},
              (int32_t)a.M, (int32_t)a.N, (int32_t)a.K, a.q_scale, a.w_scale, a.bias, a.residual, a.out, a.ldr, a.ldo,
-             (int32_t)ntn, (int32_t)(ntm * ntn), al % (4 * es) == 0};
-  launch_linear<C>(p, a.act == DPH_ACT_GELU, a.residual ? (out32 ? 2 : 1) : 0, out32, stream);
+             0, 0, al % (4 * es) == 0};
+  auto go = [&](auto c) -> int {
+    using C = decltype(c);
+    const int64_t ntm = cdiv(a.M, C::BM), ntn = cdiv(a.N, C::BN);
+    DPH_REQUIRE(ntm * ntn < (1 << 22), "dph_linear_i8: too many tiles");
+    p.ntn = (int32_t)ntn;
+    p.ntiles = (int32_t)(ntm * ntn);
+    launch_linear<C>(p, a.act == DPH_ACT_GELU, a.residual ? (out32 ? 2 : 1) : 0, out32, stream);
+    return DPH_OK;
+  };
+  const char* ev = getenv("DPH_I8_TILE");
+  const int sel = ev ? atoi(ev) : 0;
+  if (sel == 0) DPH_TRY(go(mt::Tile<128, 128, 2, 2, 2>{}));
+  if (sel == 1) DPH_TRY(go(mt::Duo<256, 256, 1>{}));
+  if (sel == 2) DPH_TRY(go(mt::Duo<128, 256, 1>{}));
+  if (sel == 3) DPH_TRY(go(mt::Duo<128, 192, 2>{}));
+  if (sel == 4) DPH_TRY(go(mt::Duo<128, 128, 2>{}));
+  if (sel == 5) DPH_TRY(go(mt::Tile<64, 64, 2, 2, 4>{}));
+  if (sel == 6) DPH_TRY(go(mt::Duo<256, 128, 1>{}));
+  if (sel == 7) DPH_TRY(go(mt::Duo<128, 192, 1>{}));
   return check_launch("dph_linear_i8");
 }

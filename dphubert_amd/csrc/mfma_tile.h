@@ -6,6 +6,10 @@
 // LDS image of an operand step: rows of 128 bytes, 16-byte chunk p of row r holds the k-chunk p ^ ((r >> 1) & 7) (no
 // bank conflict for the 16-lane groups of ds_read_b128); the swizzle is applied to the source address, since an LDS
 // DMA writes its 1 KB in lane order.
+//
+// F16T: fp16 operands that lie the other way round, sum_k A[k][m] B[k][n], so that a Gram matrix needs no transposed
+// copy: a step is 64 rows of k, the image [64][R] (R = 64 or 128 of the operand's columns), and the fragments come out
+// of it by the hardware's transposing read (ds_read_b64_tr_b16, two a fragment).
 #pragma once
 #include "gemm_core.h"
 
@@ -17,6 +21,7 @@ typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 
 struct I8 {
+  static constexpr bool TR = false;
   typedef i32x4_t acc_t;
   static constexpr int ESIZE = 1;
   static __device__ __forceinline__ acc_t mfma(i32x4_t a, i32x4_t b, acc_t c) {
@@ -24,6 +29,7 @@ struct I8 {
   }
 };
 struct F16 {
+  static constexpr bool TR = false;
   typedef f32x4_t acc_t;
   static constexpr int ESIZE = 2;
   static __device__ __forceinline__ acc_t mfma(i32x4_t a, i32x4_t b, acc_t c) {
@@ -32,20 +38,49 @@ struct F16 {
   }
 };
 
-// One operand: rows of ld bytes, `rows` of them; ld and the base are multiples of 16
+struct F16T : F16 {
+  static constexpr bool TR = true;
+};
+
+// One operand: rows of ld bytes, `rows` of them; ld and the base are multiples of 16.  F16T: `rows` columns (a multiple of
+// 8) of k-rows ld bytes apart
 struct Rows {
   const char* p;
   int64_t ld;
   int32_t rows;
 };
 
-template <int BM_, int BN_, int WR_, int WC_>
+// the transposed image [64][R]: 16-byte chunk c of k-row r stands at c ^ swz(r), which puts the 8 k-rows x 2 chunks of a
+// half-wave's transposing read on different banks
+template <int R>
+__device__ __forceinline__ int tr_swz(int r) {
+  return (2 * ((r >> 1) & 1) + 4 * ((r >> 3) & 1) + 8 * (r & 1)) & (R / 8 - 1);
+}
+// where the fragment of columns c0 .. c0 + 15 (c0 a multiple of 16) starts for a lane; substep s is 64 R bytes further
+template <int R>
+__device__ __forceinline__ int tr_off(int c0, int lane) {
+  const int i = lane & 15, q = i >> 2, p = i & 3, k0 = 8 * (lane >> 4) + q, c = (c0 >> 3) + (p >> 1);
+  return k0 * (2 * R) + ((c ^ tr_swz<R>(k0)) << 4) + ((p & 1) << 3);
+}
+template <int R>
+__device__ __forceinline__ i32x4_t tr_frag(const char* img, int off, int s) {
+  typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+  const char* p = img + off + s * 64 * R;
+  const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+  const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * R));
+  const s16x8_t v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  return __builtin_bit_cast(i32x4_t, v);
+}
+
+// WR x WC waves, a ring of S steps in the LDS
+template <int BM_, int BN_, int WR_, int WC_, int S_>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, NW = WR_ * WC_, NT = NW * 64;
+  static constexpr bool DUO = false;
+  static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, NW = WR_ * WC_, NT = NW * 64, S = S_;
   static constexpr int WTM = BM / WR, WTN = BN / WC, FM = WTM / 16, FN = WTN / 16;
   static constexpr int GA = BM / 8 / NW, GB = BN / 8 / NW;   // LDS DMA instructions of a wave per step
-  static constexpr int BUF = (BM + BN) * 128, LDS = 2 * BUF;
-  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole DMA instructions");
+  static constexpr int BUF = (BM + BN) * 128, LDS = S * BUF, WPE = 2;
+  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && 2 * LDS <= 160 * 1024, "two workgroups a CU");
 };
 
 __device__ __forceinline__ i32x4_t frag(const char* img, int row0, int s, int lane) {
@@ -66,49 +101,86 @@ __device__ __forceinline__ i32x4_t keep_bytes(i32x4_t v, int nb) {
 // acc(i, j) of wave (wr, wc), lane l: rows m0 + wr WTM + 16 i + (l & 15), columns n0 + wc WTN + 16 j + 4 (l >> 4) + r
 // (B goes in as the first operand).  Rows past the operand's end read its last row, chunks past kbytes (rounded up to
 // 16) the row's first one; where kbytes is no multiple of 128, A's bytes from kbytes on are zeroed in the registers,
-// so what stands behind a row of either operand has no effect -- for integers; fp16 rows are zero-padded to 128 bytes.
-// The product is added to acc; it ends with a barrier, so another may follow.
-template <class T, class C>
+// so what stands behind a row of either operand has no effect -- for integers; fp16 rows are zero-padded to 128 bytes,
+// F16T's k-rows to a multiple of 64 (kbytes: 2 bytes a k-row).  The product is added to what init() puts into acc while
+// the first steps are on their way; it ends with a barrier, so another may follow.  S - 1 steps are in flight: with few
+// tiles a step is a load's latency unless several are.
+template <class T, class C, class Init>
 __device__ __forceinline__ void product(const Rows& A, const Rows& B, int32_t kbytes, int32_t m0, int32_t n0,
-                                        typename T::acc_t (&acc)[C::FM][C::FN], char* smem, int wave, int lane) {
+                                        typename T::acc_t (&acc)[C::FM][C::FN], char* smem, int wave, int lane,
+                                        Init init) {
   const int wr = wave / C::WC, wc = wave % C::WC;
   const int nk = (kbytes + 127) >> 7, kend = (kbytes + 15) & ~15;
   const char *pa[C::GA], *pb[C::GB];
-  const int lrow = lane >> 3;
+  int ca[C::GA], cb[C::GB];                       // logical chunk (bytes) of this lane in its row
 #pragma unroll
-  for (int g = 0; g < C::GA; ++g) pa[g] = A.p + (int64_t)min(m0 + (g * C::NW + wave) * 8 + lrow, A.rows - 1) * A.ld;
+  for (int g = 0; g < C::GA; ++g) {
+    const int w = g * C::NW + wave;
+    if constexpr (T::TR) {
+      const int kr = w * (512 / C::BM) + lane / (C::BM / 8), c = ((lane % (C::BM / 8)) ^ tr_swz<C::BM>(kr)) * 8;
+      pa[g] = A.p + (int64_t)kr * A.ld + min(m0 + c, A.rows - 8) * 2;
+    } else {
+      const int row = w * 8 + (lane >> 3);
+      pa[g] = A.p + (int64_t)min(m0 + row, A.rows - 1) * A.ld;
+      ca[g] = ((lane & 7) ^ ((row >> 1) & 7)) << 4;
+    }
+  }
 #pragma unroll
-  for (int g = 0; g < C::GB; ++g) pb[g] = B.p + (int64_t)min(n0 + (g * C::NW + wave) * 8 + lrow, B.rows - 1) * B.ld;
-  // ((row >> 1) & 7 of row = 8 (..) + lrow)
-  auto stage = [&](int kt) {
-    char* buf = smem + (kt & 1) * C::BUF;
+  for (int g = 0; g < C::GB; ++g) {
+    const int w = g * C::NW + wave;
+    if constexpr (T::TR) {
+      const int kr = w * (512 / C::BN) + lane / (C::BN / 8), c = ((lane % (C::BN / 8)) ^ tr_swz<C::BN>(kr)) * 8;
+      pb[g] = B.p + (int64_t)kr * B.ld + min(n0 + c, B.rows - 8) * 2;
+    } else {
+      const int row = w * 8 + (lane >> 3);
+      pb[g] = B.p + (int64_t)min(n0 + row, B.rows - 1) * B.ld;
+      cb[g] = ((lane & 7) ^ ((row >> 1) & 7)) << 4;
+    }
+  }
+  auto stage = [&](int kt, int slot) {
+    char* buf = smem + slot * C::BUF;
 #pragma unroll
     for (int g = 0; g < C::GA; ++g) {
-      const int row = (g * C::NW + wave) * 8 + lrow;
-      const int off = kt * 128 + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
-      ring::dma16(reinterpret_cast<const bf16_t*>(pa[g] + (off < kend ? off : 0)), buf + (g * C::NW + wave) * 1024);
+      const char* p;
+      if constexpr (T::TR) p = pa[g] + (int64_t)kt * 64 * A.ld;
+      else p = pa[g] + (kt * 128 + ca[g] < kend ? kt * 128 + ca[g] : 0);
+      ring::dma16(reinterpret_cast<const bf16_t*>(p), buf + (g * C::NW + wave) * 1024);
     }
 #pragma unroll
     for (int g = 0; g < C::GB; ++g) {
-      const int row = (g * C::NW + wave) * 8 + lrow;
-      const int off = kt * 128 + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
-      ring::dma16(reinterpret_cast<const bf16_t*>(pb[g] + (off < kend ? off : 0)),
-                  buf + C::BM * 128 + (g * C::NW + wave) * 1024);
+      const char* p;
+      if constexpr (T::TR) p = pb[g] + (int64_t)kt * 64 * B.ld;
+      else p = pb[g] + (kt * 128 + cb[g] < kend ? kt * 128 + cb[g] : 0);
+      ring::dma16(reinterpret_cast<const bf16_t*>(p), buf + C::BM * 128 + (g * C::NW + wave) * 1024);
     }
   };
-  stage(0);
+  constexpr int G = C::GA + C::GB;
+#pragma unroll
+  for (int k = 0; k < C::S - 1; ++k)
+    if (k < nk) stage(k, k);
+  init();
+  int slot = 0;
   for (int kt = 0; kt < nk; ++kt) {
-    pp::vm_wait<0>();
+    // step kt is there: the S - 2 behind it may be in flight
+    if (nk - 1 - kt >= C::S - 2) pp::vm_wait<(C::S - 2) * G>();
+    else pp::vm_wait<0>();
     pp::bar();
-    if (kt + 1 < nk) stage(kt + 1);
-    const char* buf = smem + (kt & 1) * C::BUF;
+    // the slot that was read in the last step (every wave is past it)
+    if (kt + C::S - 1 < nk) stage(kt + C::S - 1, slot == 0 ? C::S - 1 : slot - 1);
+    const char* buf = smem + slot * C::BUF;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       i32x4_t fa[C::FM], fb[C::FN];
 #pragma unroll
-      for (int i = 0; i < C::FM; ++i) fa[i] = frag(buf, wr * C::WTM + 16 * i, s, lane);
+      for (int i = 0; i < C::FM; ++i) {
+        if constexpr (T::TR) fa[i] = tr_frag<C::BM>(buf, tr_off<C::BM>(wr * C::WTM + 16 * i, lane), s);
+        else fa[i] = frag(buf, wr * C::WTM + 16 * i, s, lane);
+      }
 #pragma unroll
-      for (int j = 0; j < C::FN; ++j) fb[j] = frag(buf + C::BM * 128, wc * C::WTN + 16 * j, s, lane);
+      for (int j = 0; j < C::FN; ++j) {
+        if constexpr (T::TR) fb[j] = tr_frag<C::BN>(buf + C::BM * 128, tr_off<C::BN>(wc * C::WTN + 16 * j, lane), s);
+        else fb[j] = frag(buf + C::BM * 128, wc * C::WTN + 16 * j, s, lane);
+      }
       if (T::ESIZE == 1 && kt * 128 + 128 > kbytes) {
         const int nb = kbytes - kt * 128 - (s * 4 + (lane >> 4)) * 16;
 #pragma unroll
@@ -120,8 +192,265 @@ __device__ __forceinline__ void product(const Rows& A, const Rows& B, int32_t kb
         for (int j = 0; j < C::FN; ++j) acc[i][j] = T::mfma(fb[j], fa[i], acc[i][j]);
     }
     pp::lgkm0();   // (this step's image is read: the next step's barrier lets it be overwritten)
+    slot = slot + 1 == C::S ? 0 : slot + 1;
   }
   pp::bar();
+}
+
+// ---- two wave groups in turn --------------------------------------------------------------------------------------
+// The same product by 8 waves, 2 along m and 4 along n, in two groups (the two rows of waves; a SIMD holds one wave of
+// each) that run one barrier interval apart: while one multiplies, the other reads its next fragments from the LDS and
+// issues the next LDS DMAs, so the matrix core and the LDS work at once.  A 128-byte step along k is staged as four
+// half-tiles with lifetimes of their own -- A-lo / A-hi: the first / last FM / 2 fragment rows of both rows of waves;
+// B-0 / B-1: the first ceil(FN / 2) / other fragment columns of every wave -- and takes four intervals:
+//   0: read B-0 (and A-lo), stage B-1(u+1); A-lo x B-0       1: read B-1, stage A-hi(u+1); A-lo x B-1
+//   2: read A-hi, stage A-lo(u+2); A-hi x B-1                3: (read A-lo(u+1)), stage B-0(u+2); A-hi x B-0
+// Every half-tile is overwritten two intervals after its last read and read one interval after the wait that retires
+// it, and one step's DMAs (G a thread) stay in flight across the barriers.  acc as product's.  A row distance of less
+// than 2^23 bytes (32-bit offsets inside a tile); fp16 rows of at least 256 bytes.
+template <int BM_, int BN_, int MINB_>
+struct Duo {
+  static constexpr bool DUO = true;
+  static constexpr int BM = BM_, BN = BN_, NW = 8, NT = 512, WC = 4;
+  static constexpr int WTM = BM / 2, WTN = BN / 4, FM = WTM / 16, FN = WTN / 16;
+  static constexpr int FM2 = FM / 2, FN0 = (FN + 1) / 2, FN1 = FN / 2;
+  static constexpr int RA = BM / 2, RB0 = 64 * FN0, RB1 = 64 * FN1;
+  static constexpr int GA = RA / 64, GB0 = RB0 / 64, GB1 = RB1 / 64, G = 2 * GA + GB0 + GB1;
+  static constexpr int O_ALO = 0, O_AHI = RA * 128, O_B0 = 2 * RA * 128, O_B1 = O_B0 + RB0 * 128;
+  static constexpr int BUF = (BM + BN) * 128, LDS = 2 * BUF;
+  static constexpr int WPE = 2 * MINB_;                    // waves per SIMD: MINB_ workgroups a CU
+  static constexpr bool SPLITA = BM_ == 256 || BN_ == 128; // A-lo of the next step is read in the last interval
+  static_assert(FM % 2 == 0 && FN >= 2 && RA % 64 == 0 && MINB_ * LDS <= 160 * 1024, "geometry");
+};
+
+template <class T, class C, class Init>
+__device__ __forceinline__ void product_duo(const Rows& A, const Rows& B, int32_t kbytes, int32_t m0, int32_t n0,
+                                            typename T::acc_t (&acc)[C::FM][C::FN], char* smem, int wave, int lane,
+                                            Init init) {
+  const int wr = wave >> 2, wc = wave & 3;
+  const int nk = max((kbytes + 127) >> 7, 2), kend = (kbytes + 15) & ~15;
+  const bool part = T::ESIZE == 1 && kbytes < nk * 128;    // (a step past kbytes: all of it masked)
+  const char* Ab = A.p + (T::TR ? (int64_t)m0 * 2 : (int64_t)m0 * A.ld);
+  const char* Bb = B.p + (T::TR ? (int64_t)n0 * 2 : (int64_t)n0 * B.ld);
+  const int32_t ml = A.rows - 1 - m0, nl = B.rows - 1 - n0, lda = (int32_t)A.ld, ldb = (int32_t)B.ld;
+  constexpr int HA = C::WTM / 2;
+  // wave instruction g * 8 + wave fills half-tile rows (g * 8 + wave) * 8 .. + 7; lane -> row lane / 8, chunk lane % 8
+  const int rw = wave * 8 + (lane >> 3);
+  const int lc = ((lane & 7) ^ ((rw >> 1) & 7)) << 4;      // ((row >> 1) & 7 does not depend on g)
+  // F16T: row rw of the half-tile image is a k-row, its chunk 8 operand columns
+  auto tr_row = [&](int g, int R) { return (g * 8 + wave) * (512 / R) + lane / (R / 8); };
+  uint32_t oal[C::GA], oah[C::GA], ob0[C::GB0], ob1[C::GB1];
+#pragma unroll
+  for (int g = 0; g < C::GA; ++g) {
+    int rho = g * 64 + rw;
+    if constexpr (T::TR) rho = ((lane % (C::RA / 8)) ^ tr_swz<C::RA>(tr_row(g, C::RA))) * 8;
+    const int row = (rho / HA) * C::WTM + rho % HA;
+    if constexpr (T::TR) {
+      const uint32_t k = (uint32_t)(tr_row(g, C::RA) * lda);
+      oal[g] = k + 2 * min(row, ml - 7);
+      oah[g] = k + 2 * min(row + HA, ml - 7);
+    } else {
+      oal[g] = (uint32_t)(min(row, ml) * lda);
+      oah[g] = (uint32_t)(min(row + HA, ml) * lda);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < C::GB0; ++g) {
+    int rho = g * 64 + rw;
+    if constexpr (T::TR) rho = ((lane % (C::RB0 / 8)) ^ tr_swz<C::RB0>(tr_row(g, C::RB0))) * 8;
+    const int row = (rho / (16 * C::FN0)) * C::WTN + rho % (16 * C::FN0);
+    if constexpr (T::TR) ob0[g] = (uint32_t)(tr_row(g, C::RB0) * ldb) + 2 * min(row, nl - 7);
+    else ob0[g] = (uint32_t)(min(row, nl) * ldb);
+  }
+#pragma unroll
+  for (int g = 0; g < C::GB1; ++g) {
+    int rho = g * 64 + rw;
+    if constexpr (T::TR) rho = ((lane % (C::RB1 / 8)) ^ tr_swz<C::RB1>(tr_row(g, C::RB1))) * 8;
+    const int row = (rho / (16 * C::FN1)) * C::WTN + 16 * C::FN0 + rho % (16 * C::FN1);
+    if constexpr (T::TR) ob1[g] = (uint32_t)(tr_row(g, C::RB1) * ldb) + 2 * min(row, nl - 7);
+    else ob1[g] = (uint32_t)(min(row, nl) * ldb);
+  }
+  auto buf = [&](int u) -> char* { return smem + (u & 1) * C::BUF; };
+  auto koff = [&](int u) -> uint32_t {
+    if (T::TR) return 0u;
+    if (T::ESIZE == 1) return u * 128 + lc < kend ? (uint32_t)(u * 128 + lc) : 0u;
+    return (uint32_t)(u * 128 + lc);
+  };
+  auto base = [&](const char* p, int64_t ld, int u) { return T::TR ? p + (int64_t)u * 64 * ld : p; };
+  auto dma = [&](const char* p, uint32_t off, char* to) { ring::dma16(reinterpret_cast<const bf16_t*>(p + off), to); };
+  auto st_alo = [&](int u) {
+    const uint32_t k = koff(u);
+    const char* p = base(Ab, A.ld, u);
+#pragma unroll
+    for (int g = 0; g < C::GA; ++g) dma(p, oal[g] + k, buf(u) + C::O_ALO + (g * 8 + wave) * 1024);
+  };
+  auto st_ahi = [&](int u) {
+    const uint32_t k = koff(u);
+    const char* p = base(Ab, A.ld, u);
+#pragma unroll
+    for (int g = 0; g < C::GA; ++g) dma(p, oah[g] + k, buf(u) + C::O_AHI + (g * 8 + wave) * 1024);
+  };
+  auto st_b0 = [&](int u) {
+    const uint32_t k = koff(u);
+    const char* p = base(Bb, B.ld, u);
+#pragma unroll
+    for (int g = 0; g < C::GB0; ++g) dma(p, ob0[g] + k, buf(u) + C::O_B0 + (g * 8 + wave) * 1024);
+  };
+  auto st_b1 = [&](int u) {
+    const uint32_t k = koff(u);
+    const char* p = base(Bb, B.ld, u);
+#pragma unroll
+    for (int g = 0; g < C::GB1; ++g) dma(p, ob1[g] + k, buf(u) + C::O_B1 + (g * 8 + wave) * 1024);
+  };
+  i32x4_t falo[C::FM2][2], fah_[C::FM2][2], fb0[C::FN0][2], fb1[C::FN1][2];
+  i32x4_t(&fahi)[C::FM2][2] = C::SPLITA ? fah_ : falo;
+  auto rd_a = [&](const char* ht, i32x4_t(&fa)[C::FM2][2]) {
+#pragma unroll
+    for (int i = 0; i < C::FM2; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (T::TR) fa[i][s] = tr_frag<C::RA>(ht, tr_off<C::RA>(wr * HA + 16 * i, lane), s);
+        else fa[i][s] = frag(ht, wr * HA + 16 * i, s, lane);
+      }
+  };
+  auto rd_b0 = [&](const char* bu) {
+#pragma unroll
+    for (int j = 0; j < C::FN0; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (T::TR) fb0[j][s] = tr_frag<C::RB0>(bu + C::O_B0, tr_off<C::RB0>(wc * 16 * C::FN0 + 16 * j, lane), s);
+        else fb0[j][s] = frag(bu + C::O_B0, wc * 16 * C::FN0 + 16 * j, s, lane);
+      }
+  };
+  auto rd_b1 = [&](const char* bu) {
+#pragma unroll
+    for (int j = 0; j < C::FN1; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (T::TR) fb1[j][s] = tr_frag<C::RB1>(bu + C::O_B1, tr_off<C::RB1>(wc * 16 * C::FN1 + 16 * j, lane), s);
+        else fb1[j][s] = frag(bu + C::O_B1, wc * 16 * C::FN1 + 16 * j, s, lane);
+      }
+  };
+  auto mask = [&](int u, i32x4_t(&fa)[C::FM2][2]) {
+    if (!part) return;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int nb = kbytes - u * 128 - (s * 4 + (lane >> 4)) * 16;
+#pragma unroll
+      for (int i = 0; i < C::FM2; ++i) fa[i][s] = keep_bytes(fa[i][s], nb);
+    }
+  };
+  auto mm0 = [&](int i0, const i32x4_t(&fa)[C::FM2][2]) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < C::FM2; ++i)
+#pragma unroll
+        for (int j = 0; j < C::FN0; ++j) acc[i0 + i][j] = T::mfma(fb0[j][s], fa[i][s], acc[i0 + i][j]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto mm1 = [&](int i0, const i32x4_t(&fa)[C::FM2][2]) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < C::FM2; ++i)
+#pragma unroll
+        for (int j = 0; j < C::FN1; ++j) acc[i0 + i][C::FN0 + j] = T::mfma(fb1[j][s], fa[i][s], acc[i0 + i][C::FN0 + j]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  constexpr int G = C::G;
+  auto go = [&]() {          // the reads of this interval are in registers
+    pp::bar();
+    pp::lgkm0();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  st_alo(0);
+  st_b0(0);
+  st_b1(0);
+  st_ahi(0);
+  st_alo(1);
+  st_b0(1);
+  init();
+  pp::vm_wait<G>();
+  pp::bar();
+  if constexpr (C::SPLITA) rd_a(buf(0) + C::O_ALO, falo);
+  if (wr == 1) pp::bar();    // group 1 runs one interval behind group 0
+  int u = 0;
+#pragma unroll 1
+  for (; u + 2 < nk; ++u) {
+    const char* bu = buf(u);
+    rd_b0(bu);
+    if constexpr (!C::SPLITA) rd_a(bu + C::O_ALO, falo);
+    st_b1(u + 1);
+    pp::vm_wait<G>();
+    go();
+    mm0(0, falo);
+    pp::bar();
+    rd_b1(bu);
+    st_ahi(u + 1);
+    pp::vm_wait<G>();
+    go();
+    mm1(0, falo);
+    pp::bar();
+    rd_a(bu + C::O_AHI, fahi);
+    st_alo(u + 2);
+    pp::vm_wait<G>();
+    go();
+    mm1(C::FM2, fahi);
+    pp::bar();
+    if constexpr (C::SPLITA) rd_a(buf(u + 1) + C::O_ALO, falo);
+    st_b0(u + 2);
+    pp::vm_wait<G>();
+    pp::bar();
+    mm0(C::FM2, fahi);
+    pp::bar();
+  }
+  // the last two steps: nothing is staged past nk - 1, the waits drain
+#pragma unroll
+  for (int t = 0; t < 2; ++t, ++u) {
+    const char* bu = buf(u);
+    rd_b0(bu);
+    if constexpr (!C::SPLITA) rd_a(bu + C::O_ALO, falo);
+    if (t == 0) {
+      st_b1(u + 1);
+      pp::vm_wait<G>();
+    } else {
+      pp::vm_wait<C::GA>();
+    }
+    go();
+    mask(u, falo);
+    mm0(0, falo);
+    pp::bar();
+    rd_b1(bu);
+    if (t == 0) {
+      st_ahi(u + 1);
+      pp::vm_wait<G>();
+    } else {
+      pp::vm_wait<0>();
+    }
+    go();
+    mm1(0, falo);
+    pp::bar();
+    rd_a(bu + C::O_AHI, fahi);
+    if (t == 0) pp::vm_wait<G - C::GA>();
+    else pp::vm_wait<0>();
+    go();
+    mask(u, fahi);
+    mm1(C::FM2, fahi);
+    pp::bar();
+    if (t == 0) {
+      if constexpr (C::SPLITA) rd_a(buf(u + 1) + C::O_ALO, falo);
+      pp::vm_wait<C::GB1 + C::GA>();
+    } else {
+      pp::vm_wait<0>();
+    }
+    pp::bar();
+    mm0(C::FM2, fahi);
+    pp::bar();
+  }
+  if (wr == 0) pp::bar();    // pairs with group 1's first one
 }
 
 template <class T, class C>
@@ -131,6 +460,56 @@ __device__ __forceinline__ void clear(typename T::acc_t (&acc)[C::FM][C::FN]) {
 #pragma unroll
     for (int j = 0; j < C::FN; ++j) acc[i][j] = typename T::acc_t{0, 0, 0, 0};
 }
+
+template <class T, class C, class Init>
+__device__ __forceinline__ void product_of(const Rows& A, const Rows& B, int32_t kbytes, int32_t m0, int32_t n0,
+                                           typename T::acc_t (&acc)[C::FM][C::FN], char* smem, int wave, int lane,
+                                           Init init) {
+  if constexpr (C::DUO) product_duo<T, C>(A, B, kbytes, m0, n0, acc, smem, wave, lane, init);
+  else product<T, C>(A, B, kbytes, m0, n0, acc, smem, wave, lane, init);
+}
+
+// ---- whole rows in a lane --------------------------------------------------------------------------------------------
+// A wave's 16 x 16 FN strip of acc has 4 columns of each fragment in a lane: 8-byte accesses of 32-byte runs.  Exchanging
+// them between the four groups of 16 lanes (a transpose of groups and fragments, by lane swaps; its own inverse) gives a
+// lane W = 16 (8 where FN = 2) consecutive columns, and a row of the wave 128-byte runs of fp16.
+template <int FN>
+struct Strip {
+  static constexpr int W = FN % 4 == 0 ? 16 : 8, NG = 4 * FN / W;   // NG groups of W columns a lane
+  static_assert(FN % 4 == 0 || FN == 2, "whole exchanges");
+  // first column of group q in the strip
+  static __device__ __forceinline__ int col(int q, int lane) {
+    return W == 16 ? 64 * q + 16 * (lane >> 4) : 16 * ((lane >> 4) & 1) + 8 * (lane >> 5);
+  }
+  static __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+  }
+  static __device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+  }
+  // v[4 j + r]: fragment j's column 4 (lane / 16) + r  <->  v[W q + c]: column col(q) + c
+  static __device__ __forceinline__ void exchange(uint32_t (&v)[4 * FN]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (W == 16) {
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+          uint32_t* a = v + 16 * q + r;
+          swap32(a[0], a[8]);
+          swap32(a[4], a[12]);
+          swap16(a[0], a[4]);
+          swap16(a[8], a[12]);
+        }
+      } else {
+        swap16(v[r], v[4 + r]);
+      }
+    }
+  }
+};
 
 // Workgroups go to the 8 XCDs in turn: block b of n works on a contiguous range of tiles per XCD, so the tiles of one
 // L2 share their operands' rows

@@ -11,15 +11,22 @@
 // Two things keep the operands' rounding (2^-12) from growing through the steps; rounding errors of the result against
 // 64 bits (2-norm, 5 steps, sizes 64 to 1533, of noise / of a few directions 100 times above the rest): plain fp16
 // 1.3e-3 / 1.1e-2, as built 0.8e-3 / 1.3e-3, bf16 in place of fp16 1.0e-2 / 9e-2.
-//   * While singular values grow, a X dominates the step: X is held as two fp16 (22 bits) for that term, so weak
-//     directions are not lost in the rounding of strong ones.  The products read the upper half alone.
+//   * While singular values grow, a X dominates the step: X is held in 16 bits and more for that term (fp16, and what it
+//     leaves in e4m3), so weak directions are not lost in the rounding of strong ones.  The products read the fp16 alone.
 //   * In the last two steps the singular values are near 1 and a X + b A X + c A^2 X cancel by a factor of 5.  There the
 //     polynomial is expanded about d = 1:  E = A - d I,  F = (b + 2 c d) E + c E^2,  X <- (a + b d + c d^2) X + F X,
 //     the same products on numbers near 0, whose roundings are small.
 // In large matrices an operand's roundings average out; up to NS_SPLIT rows they need not (a 1 x 1 matrix is off by
-// 8e-3), and there every operand is two fp16 and every product three: h h + l h + h l.  Such a matrix is one row of
-// tiles: launches, not products, set its time.
+// 8e-3), and there every operand is two fp16 and every product three: h h + l h + h l.  Such matrices are a few tiles:
+// launches, not products, set their time.
+//
+// Layout.  What is stored is Y = X^T ([n][m], the long side first), and only that: Y F has both operands contiguous
+// along k, and the Gram matrix reads Y through the transposing LDS read.  A step then moves Y in and out once (and its 8
+// more bits while they are held) -- with a transposed copy kept, and 16 bits more, the update of 24 matrices of 4096 x
+// 1024 wrote 600 MB and took 487 us at 850 TFLOP/s.
 #include "mfma_tile.h"
+
+#include <type_traits>
 
 
 namespace dph {
@@ -35,25 +42,43 @@ constexpr int NS_SPLIT = 128;      // rows up to which all operands are held in 
 __device__ __forceinline__ f16_t f2h(float v) { return __builtin_bit_cast(f16_t, (_Float16)v); }
 __device__ __forceinline__ float h2f(f16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
 __device__ __forceinline__ uint32_t pack2h(float a, float b) { return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16); }
-__device__ __forceinline__ void unpack4h(uint2 r, float (&v)[4]) {
+__device__ __forceinline__ void unpack4h(uint2 r, float* v) {
   v[0] = h2f((f16_t)(r.x & 0xffff)); v[1] = h2f((f16_t)(r.x >> 16));
   v[2] = h2f((f16_t)(r.y & 0xffff)); v[3] = h2f((f16_t)(r.y >> 16));
 }
 
-// what 4 numbers have beyond their fp16 halves h
-__device__ __forceinline__ uint2 low4h(const float (&v)[4], uint2 h) {
+// what 4 numbers have beyond their fp16 halves h, as fp16
+__device__ __forceinline__ uint2 low4h(const float* v, uint2 h) {
   float q[4];
   unpack4h(h, q);
   return make_uint2(pack2h(v[0] - q[0], v[1] - q[1]), pack2h(v[2] - q[2], v[3] - q[3]));
 }
+// the same in e4m3, times 2^13: half a place of a mean entry (1/4) counts 1/2; what entries above 900 times that leave is
+// cut off at e4m3's 448
+constexpr float LO_UP = 8192.f;
+__device__ __forceinline__ uint32_t low4q(const float* v, uint2 h) {
+  float q[4];
+  unpack4h(h, q);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) q[r] = fminf(fmaxf((v[r] - q[r]) * LO_UP, -448.f), 448.f);
+  const int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+}
+__device__ __forceinline__ void add_low4q(float* v, uint32_t w) {
+  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  v[0] += a[0] * (1.f / LO_UP);
+  v[1] += a[1] * (1.f / LO_UP);
+  v[2] += b[0] * (1.f / LO_UP);
+  v[3] += b[1] * (1.f / LO_UP);
+}
 
-// Matrices of one shape: cnt of them, each m x n (m <= n) in rows padded with zeros to multiples of 64 (mp, np)
+// Matrices of one shape: cnt of them, Y n x m (m <= n) in rows padded with zeros to multiples of 64 (np, mp)
 struct Group {
-  int32_t m, n, mp, np, cnt, trans;   // trans: the caller's matrices are n x m
-  float s;                            // X is held times s
+  int32_t m, n, mp, np, cnt, wide;    // wide: the caller's matrices are m x n
+  float s;                            // Y is held times s
   int32_t in_f32;
-  char *xh, *xl, *xt[2], *e, *f;      // [cnt][mp][np] x 2, [cnt][np][mp] x 2, [cnt][mp][mp] x 2
-  char *xtl[2], *el, *fl;             // the lower halves of xt, e, f (split) or null
+  char *y[2], *lo, *yl[2];            // [cnt][np][mp]: fp16 x 2, then e4m3, or (split) two fp16 halves more
+  char *e, *f, *el, *fl;              // [cnt][mp][mp]; the lower halves (split) or null
   double* part;                       // [cnt][NS_PARTS]
   bf16_t* out;                        // [cnt] matrices as the caller has them, dense
 };
@@ -64,7 +89,7 @@ struct Groups {
 };
 struct Mat {
   const void* p;
-  int64_t rs, cs;                     // strides of the row and the column index of the m x n orientation
+  int64_t ns, ms;                     // strides of Y's row and column index; one of them is 1
   int32_t group, index, first, pad;   // group, place in it, first block of the launch
 };
 struct Mats {
@@ -72,15 +97,14 @@ struct Mats {
   Mat m[NS_MATS];
 };
 struct Step {
-  float d, fe, fq, mu;     // E = A - d I;  F = fe E + fq E^2;  X <- mu X + F X
-  int32_t cur;             // which xt is read
-  int32_t lo_in, lo_out;   // X's lower half is read, written
+  float d, fe, fq, mu;     // E = A - d I;  F = fe E + fq E^2;  Y <- mu Y + Y F
+  int32_t cur;             // which y is read
+  int32_t lo_in, lo_out;   // Y's 8 bits more are read, written
 };
-
 struct PackGroup {
   int32_t m, n, mp, np, in_f32;
   float s;
-  char *xh, *xl, *xt, *xtl;
+  char *y, *lo, *yl;
   double* part;
 };
 struct PackGroups {
@@ -98,24 +122,57 @@ __device__ __forceinline__ int find_mat(const Mats& a, int b) {
   return k;
 }
 
-// Sums of squares in 64 bits, NS_PARTS strips of rows a matrix (in its memory order), added in a fixed order later
+// Sums of squares in 64 bits, NS_PARTS parts of a matrix, added in a fixed order later.  A matrix without gaps is read
+// as one run of 16-byte vectors, another line by line.
 __global__ void __launch_bounds__(256) ns_sumsq_kernel(const Mats a, const PackGroups pg) {
   const int k = find_mat(a, (int)blockIdx.x);
   const Mat& t = a.m[k];
   const PackGroup& g = pg.g[t.group];
   const int part = (int)blockIdx.x - t.first;
-  // walk along the unit stride
-  const bool by_row = t.cs == 1;
-  const int32_t R = by_row ? g.m : g.n, L = by_row ? g.n : g.m;
-  const int64_t rs = by_row ? t.rs : t.cs, cs = by_row ? t.cs : t.rs;
-  double s = 0.0;
-  const int64_t total = (int64_t)R * L, per = cdiv(total, NS_PARTS);
-  const int64_t i1 = min(total, (part + 1) * per);
-  for (int64_t i = part * per + threadIdx.x; i < i1; i += 256) {
-    const int64_t r = i / L, c = i - r * L;
-    const double v = ldg(t.p, r * rs + c * cs, g.in_f32);
-    s += v * v;
+  const bool by_n = t.ms == 1;
+  const int64_t lines = by_n ? g.n : g.m, len = by_n ? g.m : g.n, gap = by_n ? t.ns : t.ms;
+  const int esize = g.in_f32 ? 4 : 2, ve = 16 / esize;
+  double s0 = 0.0, s1 = 0.0;
+  auto add4 = [&](float4 v) {
+    s0 += (double)v.x * v.x + (double)v.y * v.y;
+    s1 += (double)v.z * v.z + (double)v.w * v.w;
+  };
+  if (gap == len && (reinterpret_cast<uintptr_t>(t.p) & 15) == 0) {
+    const int64_t total = lines * len, nv = total / ve, per = cdiv(nv, NS_PARTS);
+    const int64_t i1 = min(nv, (part + 1) * per);
+    const uint4* p = reinterpret_cast<const uint4*>(t.p);
+    auto add = [&](uint4 r) {
+      if (g.in_f32) {
+        add4(make_float4(__uint_as_float(r.x), __uint_as_float(r.y), __uint_as_float(r.z), __uint_as_float(r.w)));
+      } else {
+        add4(make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16),
+                         __uint_as_float(r.y & 0xffff0000u)));
+        add4(make_float4(__uint_as_float(r.z << 16), __uint_as_float(r.z & 0xffff0000u), __uint_as_float(r.w << 16),
+                         __uint_as_float(r.w & 0xffff0000u)));
+      }
+    };
+    int64_t i = part * per + threadIdx.x;
+    for (; i + 768 < i1; i += 1024) {
+      const uint4 r0 = p[i], r1 = p[i + 256], r2 = p[i + 512], r3 = p[i + 768];
+      add(r0);
+      add(r1);
+      add(r2);
+      add(r3);
+    }
+    for (; i < i1; i += 256) add(p[i]);
+    if (part == NS_PARTS - 1)
+      for (int64_t q = nv * ve + threadIdx.x; q < total; q += 256) {
+        const double v = ldg(t.p, q, g.in_f32);
+        s0 += v * v;
+      }
+  } else {
+    for (int64_t l = part; l < lines; l += NS_PARTS)
+      for (int64_t q = threadIdx.x; q < len; q += 256) {
+        const double v = ldg(t.p, l * gap + q, g.in_f32);
+        s0 += v * v;
+      }
   }
+  double s = s0 + s1;
   __shared__ double red[4];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -124,7 +181,7 @@ __global__ void __launch_bounds__(256) ns_sumsq_kernel(const Mats a, const PackG
   if (threadIdx.x == 0) g.part[(int64_t)t.index * NS_PARTS + part] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// X0 in both orders, 64 x 64 tiles through the LDS; reads run along whichever stride of the input is 1
+// Y0, 64 x 64 tiles through the LDS; reads run along whichever stride of the input is 1
 __global__ void __launch_bounds__(256) ns_pack_kernel(const Mats a, const PackGroups pg, float eps) {
   __shared__ float tile[64][65];
   __shared__ float scale;
@@ -137,41 +194,33 @@ __global__ void __launch_bounds__(256) ns_pack_kernel(const Mats a, const PackGr
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if (threadIdx.x == 0) scale = (float)((double)g.s / (sqrt(s) + (double)eps));
   }
-  const int b = (int)blockIdx.x - t.first, tn = g.np >> 6;
-  const int r0 = b / tn * 64, c0 = b % tn * 64;
-  __syncthreads();
-  const float sc = scale;
+  const int b = (int)blockIdx.x - t.first, tm = g.mp >> 6;
+  const int r0 = b / tm * 64, c0 = b % tm * 64;
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  if (t.cs == 1) {
-    for (int i = ty; i < 64; i += 4)
-      tile[i][tx] = r0 + i < g.m && c0 + tx < g.n ? ldg(t.p, (int64_t)(r0 + i) * t.rs + c0 + tx, g.in_f32) * sc : 0.f;
-  } else {
-    for (int i = ty; i < 64; i += 4)
-      tile[tx][i] = r0 + tx < g.m && c0 + i < g.n ? ldg(t.p, (int64_t)(r0 + tx) * t.rs + (int64_t)(c0 + i) * t.cs, g.in_f32) * sc : 0.f;
+  float in[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = r0 + (t.ms == 1 ? 4 * i + ty : tx), c = c0 + (t.ms == 1 ? tx : 4 * i + ty);
+    in[i] = r < g.n && c < g.m ? ldg(t.p, r * t.ns + c * t.ms, g.in_f32) : 0.f;
   }
   __syncthreads();
-  const int64_t mat = (int64_t)t.index * g.mp * g.np;
-  // 4 consecutive elements a thread
-  const int x4 = (threadIdx.x & 15) * 4, y = threadIdx.x >> 4;
-  for (int i = y; i < 64; i += 16) {
-    float v[4], lo[4];
+  const float sc = scale;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = tile[i][x4 + j];
-      lo[j] = v[j] - h2f(f2h(v[j]));
-    }
-    const int64_t o = mat + (int64_t)(r0 + i) * g.np + c0 + x4;
-    *reinterpret_cast<uint2*>(reinterpret_cast<f16_t*>(g.xh) + o) = make_uint2(pack2h(v[0], v[1]), pack2h(v[2], v[3]));
-    *reinterpret_cast<uint2*>(reinterpret_cast<f16_t*>(g.xl) + o) = make_uint2(pack2h(lo[0], lo[1]), pack2h(lo[2], lo[3]));
-    const int64_t ot = mat + (int64_t)(c0 + i) * g.mp + r0 + x4;
+  for (int i = 0; i < 16; ++i) {
+    if (t.ms == 1) tile[4 * i + ty][tx] = in[i] * sc;
+    else tile[tx][4 * i + ty] = in[i] * sc;
+  }
+  __syncthreads();
+  const int64_t mat = (int64_t)t.index * g.np * g.mp;
+  const int x4 = (threadIdx.x & 15) * 4;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = tile[x4 + j][i];
-      lo[j] = v[j] - h2f(f2h(v[j]));
-    }
-    *reinterpret_cast<uint2*>(reinterpret_cast<f16_t*>(g.xt) + ot) = make_uint2(pack2h(v[0], v[1]), pack2h(v[2], v[3]));
-    if (g.xtl)
-      *reinterpret_cast<uint2*>(reinterpret_cast<f16_t*>(g.xtl) + ot) = make_uint2(pack2h(lo[0], lo[1]), pack2h(lo[2], lo[3]));
+  for (int i = threadIdx.x >> 4; i < 64; i += 16) {
+    const float v[4] = {tile[i][x4], tile[i][x4 + 1], tile[i][x4 + 2], tile[i][x4 + 3]};
+    const int64_t o = mat + (int64_t)(r0 + i) * g.mp + c0 + x4;
+    const uint2 h = make_uint2(pack2h(v[0], v[1]), pack2h(v[2], v[3]));
+    *reinterpret_cast<uint2*>(g.y + 2 * o) = h;
+    if (g.yl) *reinterpret_cast<uint2*>(g.yl + 2 * o) = low4h(v, h);
+    else *reinterpret_cast<uint32_t*>(g.lo + o) = low4q(v, h);
   }
 }
 
@@ -191,21 +240,21 @@ __device__ __forceinline__ uint2 quad_transpose(uint2 x, int lane) {
   return o2 ? make_uint2(b1, a1) : make_uint2(a0, b0);
 }
 
-template <int KIND, class C>
-__global__ void __launch_bounds__(C::NT, 2) ns_product_kernel(const Groups gs, const Step st) {
+template <int KIND, bool SPLIT, class C>
+__global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups gs, const Step st) {
   __shared__ __align__(16) char smem[C::LDS];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   int t = mt::xcd_tile((int)blockIdx.x, (int)gridDim.x);
   int k = 0;
   while (k + 1 < gs.ng && gs.first[k + 1] <= t) ++k;
   const Group& g = gs.g[k];
   t -= gs.first[k];
   constexpr bool SYM = KIND == GRAM || KIND == POLY;
-  const int tm = (g.m + C::BM - 1) / C::BM;
+  using T = std::conditional_t<KIND == GRAM, mt::F16T, mt::F16>;
   int ti, tj, z;
   if (SYM) {
-    static_assert(C::BM == C::BN && C::BM >= NS_SPLIT, "square tiles, one of them where operands are split");
-    const int per = tm * (tm + 1) / 2;
+    static_assert(!SYM || C::BM == C::BN, "square tiles");
+    const int tm = (g.m + C::BM - 1) / C::BM, per = tm * (tm + 1) / 2;
     z = t / per;
     t -= z * per;
     ti = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
@@ -213,115 +262,181 @@ __global__ void __launch_bounds__(C::NT, 2) ns_product_kernel(const Groups gs, c
     while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
     tj = t - ti * (ti + 1) / 2;
   } else {
-    const int tn = (g.n + C::BN - 1) / C::BN, per = tm * tn;
+    const int tm = (g.m + C::BN - 1) / C::BN, tn = (g.n + C::BM - 1) / C::BM, per = tm * tn;
     z = t / per;
     t -= z * per;
-    tj = t / tm;         // (consecutive tiles share rows of X^T)
-    ti = t % tm;
+    ti = t / tm;         // (consecutive tiles share rows of Y)
+    tj = t % tm;
   }
   const int m0 = ti * C::BM, n0 = tj * C::BN;
-  const int64_t xoff = (int64_t)z * g.mp * g.np * 2, eoff = (int64_t)z * g.mp * g.mp * 2;
-  const bool split = g.el != nullptr;
+  const int64_t yoff = (int64_t)z * g.np * g.mp * 2, eoff = (int64_t)z * g.mp * g.mp * 2;
+  const int kbytes = (KIND == GRAM ? g.np : g.mp) * 2;
+  const int64_t ld = (int64_t)g.mp * 2;
+  using V = mt::Strip<C::FN>;
+  constexpr int NV = 4 * C::FN;
   f32x4_t acc[C::FM][C::FN];
-  mt::clear<mt::F16, C>(acc);
-  for (int part = 0; part < (split ? 3 : 1); ++part) {   // h h, l h, h l
+  const int mw = m0 + wave / C::WC * C::WTM + (lane & 15), nw = n0 + wave % C::WC * C::WTN;
+  const int M = SYM ? g.mp : g.np, N = g.mp;      // (what lies past m and n is zero, and stays zero)
+  // the sums start from 0, or from mu Y, whose rows are about to be read as an operand anyway
+  auto init = [&]() {
+    if constexpr (SYM) {
+      mt::clear<T, C>(acc);
+    } else {
+      const float mu = st.mu * NS_E;
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) {
+        const int m = mw + 16 * i;
+        float x[NV];
+#pragma unroll
+        for (int q = 0; q < V::NG; ++q) {
+          const int n = nw + V::col(q, lane);
+          const bool in = m < M && n < N;
+          const int64_t o = yoff / 2 + (int64_t)m * N + n;
+#pragma unroll
+          for (int c = 0; c < V::W; c += 8) {
+            const uint4 h = in ? *reinterpret_cast<const uint4*>(g.y[st.cur] + 2 * (o + c)) : make_uint4(0, 0, 0, 0);
+            unpack4h(make_uint2(h.x, h.y), x + V::W * q + c);
+            unpack4h(make_uint2(h.z, h.w), x + V::W * q + c + 4);
+            if (SPLIT) {
+              const uint4 l = in ? *reinterpret_cast<const uint4*>(g.yl[st.cur] + 2 * (o + c)) : make_uint4(0, 0, 0, 0);
+              float lo[8];
+              unpack4h(make_uint2(l.x, l.y), lo);
+              unpack4h(make_uint2(l.z, l.w), lo + 4);
+#pragma unroll
+              for (int r = 0; r < 8; ++r) x[V::W * q + c + r] += lo[r];
+            } else if (st.lo_in) {
+              const uint2 l = in ? *reinterpret_cast<const uint2*>(g.lo + o + c) : make_uint2(0, 0);
+              add_low4q(x + V::W * q + c, l.x);
+              add_low4q(x + V::W * q + c + 4, l.y);
+            }
+          }
+        }
+        uint32_t b[NV];
+#pragma unroll
+        for (int r = 0; r < NV; ++r) b[r] = __float_as_uint(x[r] * mu);
+        V::exchange(b);
+#pragma unroll
+        for (int r = 0; r < NV; ++r) acc[i][r >> 2][r & 3] = __uint_as_float(b[r]);
+      }
+    }
+  };
+#pragma unroll 1
+  for (int part = 0; part < (SPLIT ? 3 : 1); ++part) {   // h h, l h, h l
     const bool la = part == 1, lb = part == 2;
     mt::Rows A, B;
-    int kbytes;
     if constexpr (KIND == GRAM) {
-      kbytes = g.np * 2;
-      A = mt::Rows{(la ? g.xl : g.xh) + xoff, kbytes, g.mp};
-      B = mt::Rows{(lb ? g.xl : g.xh) + xoff, kbytes, g.mp};
+      A = mt::Rows{(la ? g.yl[st.cur] : g.y[st.cur]) + yoff, ld, g.mp};
+      B = mt::Rows{(lb ? g.yl[st.cur] : g.y[st.cur]) + yoff, ld, g.mp};
     } else if constexpr (KIND == POLY) {
-      kbytes = g.mp * 2;
-      A = mt::Rows{(la ? g.el : g.e) + eoff, kbytes, g.mp};
-      B = mt::Rows{(lb ? g.el : g.e) + eoff, kbytes, g.mp};
+      A = mt::Rows{(la ? g.el : g.e) + eoff, ld, g.mp};
+      B = mt::Rows{(lb ? g.el : g.e) + eoff, ld, g.mp};
     } else {
-      kbytes = g.mp * 2;
-      A = mt::Rows{(la ? g.fl : g.f) + eoff, kbytes, g.mp};
-      B = mt::Rows{(lb ? g.xtl[st.cur] : g.xt[st.cur]) + xoff, kbytes, g.np};
+      A = mt::Rows{(la ? g.yl[st.cur] : g.y[st.cur]) + yoff, ld, g.np};
+      B = mt::Rows{(lb ? g.fl : g.f) + eoff, ld, g.mp};
     }
-    mt::product<mt::F16, C>(A, B, kbytes, m0, n0, acc, smem, wave, lane);
+    mt::product_of<T, C>(A, B, kbytes, m0, n0, acc, smem, wave, lane, [&]() {
+      if (!SPLIT || part == 0) init();
+    });
   }
 
-  const int ml = m0 + wave / C::WC * C::WTM + (lane & 15), nl = n0 + wave % C::WC * C::WTN + 4 * (lane >> 4);
-  const int M = g.mp, N = SYM ? g.mp : g.np;      // (what lies past m and n is zero, and stays zero)
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
+    const int m = mw + 16 * i;
+    uint32_t b[NV];
 #pragma unroll
-    for (int j = 0; j < C::FN; ++j) {
-      const int m = ml + 16 * i, n = nl + 16 * j;
-      const bool in = m < M && n < N;
-      // rows of the quad's transpose: n + (lane & 3), columns 4 (m / 4) ..
-      const int tr = n + (lane & 3), tc = m & ~3;
-      float v[4];
+    for (int r = 0; r < NV; ++r) b[r] = __float_as_uint(acc[i][r >> 2][r & 3]);
+    V::exchange(b);
+#pragma unroll
+    for (int q = 0; q < V::NG; ++q) {
+      const int n0q = nw + V::col(q, lane);
+      const bool in = m < M && n0q < N;
+      float v[V::W];
+      uint2 h[V::W / 4];
+#pragma unroll
+      for (int r = 0; r < V::W; ++r) v[r] = __uint_as_float(b[V::W * q + r]);
       if constexpr (SYM) {
+        char* to = (KIND == GRAM ? g.e : g.f) + eoff;
+        char* tl = (KIND == GRAM ? g.el : g.fl) + eoff;
+        const int64_t o = (int64_t)m * N + n0q;
         if constexpr (KIND == GRAM) {
           const float sc = NS_E / (g.s * g.s);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * sc - (m == n + r && m < g.m ? NS_E * st.d : 0.f);
+          for (int r = 0; r < V::W; ++r) v[r] = v[r] * sc - (m == n0q + r && m < g.m ? NS_E * st.d : 0.f);
         } else {
-          float e[4] = {0.f, 0.f, 0.f, 0.f};
-          if (in) {
-            unpack4h(*reinterpret_cast<const uint2*>(g.e + eoff + ((int64_t)m * M + n) * 2), e);
-            if (split) {
-              float lo[4];
-              unpack4h(*reinterpret_cast<const uint2*>(g.el + eoff + ((int64_t)m * M + n) * 2), lo);
 #pragma unroll
-              for (int r = 0; r < 4; ++r) e[r] += lo[r];
+          for (int r = 0; r < V::W; ++r) v[r] *= st.fq / NS_E;
+#pragma unroll
+          for (int c = 0; c < V::W; c += 4) {
+            float e[4] = {0.f, 0.f, 0.f, 0.f};
+            if (in) {
+              unpack4h(*reinterpret_cast<const uint2*>(g.e + eoff + (o + c) * 2), e);
+              if constexpr (SPLIT) {
+                float lo[4];
+                unpack4h(*reinterpret_cast<const uint2*>(g.el + eoff + (o + c) * 2), lo);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) e[r] += lo[r];
+              }
             }
-          }
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = st.fe * e[r] + st.fq / NS_E * acc[i][j][r];
+            for (int r = 0; r < 4; ++r) v[c + r] += st.fe * e[r];
+          }
         }
-        const uint2 h = make_uint2(pack2h(v[0], v[1]), pack2h(v[2], v[3]));
-        char* o = (KIND == GRAM ? g.e : g.f) + eoff;
-        if (in) *reinterpret_cast<uint2*>(o + ((int64_t)m * M + n) * 2) = h;
-        const uint2 ht = quad_transpose(h, lane);
-        if (ti != tj && in) *reinterpret_cast<uint2*>(o + ((int64_t)tr * M + tc) * 2) = ht;
-        if (split && in)       // (a single tile: its own mirror image)
-          *reinterpret_cast<uint2*>((KIND == GRAM ? g.el : g.fl) + eoff + ((int64_t)m * M + n) * 2) = low4h(v, h);
-      } else {
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        const int64_t o = xoff + ((int64_t)m * N + n) * 2;
+#pragma unroll
+        for (int c = 0; c < V::W / 4; ++c) {
+          h[c] = make_uint2(pack2h(v[4 * c], v[4 * c + 1]), pack2h(v[4 * c + 2], v[4 * c + 3]));
+          const uint2 ht = quad_transpose(h[c], lane);
+          const int64_t ot = (int64_t)(n0q + 4 * c + (lane & 3)) * M + (m & ~3);
+          if (ti != tj && in) *reinterpret_cast<uint2*>(to + ot * 2) = ht;
+          if constexpr (SPLIT) {
+            const uint2 l = low4h(v + 4 * c, h[c]), lt = quad_transpose(l, lane);
+            if (in) *reinterpret_cast<uint2*>(tl + (o + 4 * c) * 2) = l;
+            if (ti != tj && in) *reinterpret_cast<uint2*>(tl + ot * 2) = lt;
+          }
+        }
         if (in) {
-          unpack4h(*reinterpret_cast<const uint2*>(g.xh + o), x);
-          if (st.lo_in || split) {
-            float lo[4];
-            unpack4h(*reinterpret_cast<const uint2*>(g.xl + o), lo);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] += lo[r];
+          for (int c = 0; c < V::W / 4; c += 2)
+            *reinterpret_cast<uint4*>(to + (o + 4 * c) * 2) = make_uint4(h[c].x, h[c].y, h[c + 1].x, h[c + 1].y);
+        }
+      } else if constexpr (KIND == UPDATE) {
+        if (in) {
+          const int64_t o = yoff / 2 + (int64_t)m * N + n0q;
+          uint32_t l[V::W / 4];
+#pragma unroll
+          for (int r = 0; r < V::W; ++r) v[r] *= 1.f / NS_E;
+#pragma unroll
+          for (int c = 0; c < V::W / 4; ++c) {
+            h[c] = make_uint2(pack2h(v[4 * c], v[4 * c + 1]), pack2h(v[4 * c + 2], v[4 * c + 3]));
+            if constexpr (SPLIT) *reinterpret_cast<uint2*>(g.yl[st.cur ^ 1] + 2 * (o + 4 * c)) = low4h(v + 4 * c, h[c]);
+            else if (st.lo_out) l[c] = low4q(v + 4 * c, h[c]);
+          }
+#pragma unroll
+          for (int c = 0; c < V::W / 4; c += 2)
+            *reinterpret_cast<uint4*>(g.y[st.cur ^ 1] + 2 * (o + 4 * c)) =
+                make_uint4(h[c].x, h[c].y, h[c + 1].x, h[c + 1].y);
+          if (!SPLIT && st.lo_out) {
+            if constexpr (V::W == 16) *reinterpret_cast<uint4*>(g.lo + o) = make_uint4(l[0], l[1], l[2], l[3]);
+            else *reinterpret_cast<uint2*>(g.lo + o) = make_uint2(l[0], l[1]);
           }
         }
+      } else {
+        const float inv = 1.0f / (g.s * NS_E);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = st.mu * x[r] + acc[i][j][r] / NS_E;
-        if constexpr (KIND == UPDATE) {
-          const uint2 h = make_uint2(pack2h(v[0], v[1]), pack2h(v[2], v[3]));
-          if (in) {
-            *reinterpret_cast<uint2*>(g.xh + o) = h;
-            if (st.lo_out || split) *reinterpret_cast<uint2*>(g.xl + o) = low4h(v, h);
-          }
-          const uint2 ht = quad_transpose(h, lane);
-          if (in) *reinterpret_cast<uint2*>(g.xt[st.cur ^ 1] + xoff + ((int64_t)tr * g.mp + tc) * 2) = ht;
-          if (split) {
-            const uint2 lt = quad_transpose(low4h(v, h), lane);
-            if (in) *reinterpret_cast<uint2*>(g.xtl[st.cur ^ 1] + xoff + ((int64_t)tr * g.mp + tc) * 2) = lt;
-          }
-        } else {
-          const float inv = 1.0f / g.s;
-          uint2 h = make_uint2(pack2bf(v[0] * inv, v[1] * inv), pack2bf(v[2] * inv, v[3] * inv));
-          // the caller's order: rows of n, or of m where the matrix was transposed
-          int row = m, col = n, cols = g.n, rows = g.m;
-          if (g.trans) {
-            h = quad_transpose(h, lane);
-            row = tr, col = tc, cols = g.m, rows = g.n;
+        for (int c = 0; c < V::W / 4; ++c) {
+          const int n = n0q + 4 * c;
+          h[c] = make_uint2(pack2bf(v[4 * c] * inv, v[4 * c + 1] * inv), pack2bf(v[4 * c + 2] * inv, v[4 * c + 3] * inv));
+          // the caller's order: rows of m, or of n where the matrix is wide
+          int row = m, col = n, cols = g.m, rows = g.n;
+          if (g.wide) {
+            h[c] = quad_transpose(h[c], lane);
+            row = n + (lane & 3), col = m & ~3, cols = g.n, rows = g.m;
           }
           bf16_t* p = g.out + (int64_t)z * g.m * g.n + (int64_t)row * cols + col;
           if (row < rows) {
             if (col + 4 <= cols && (cols & 3) == 0) {
-              *reinterpret_cast<uint2*>(p) = h;
+              *reinterpret_cast<uint2*>(p) = h[c];
             } else {
-              const uint32_t w[2] = {h.x, h.y};
+              const uint32_t w[2] = {h[c].x, h[c].y};
 #pragma unroll
               for (int r = 0; r < 4; ++r)
                 if (col + r < cols) p[r] = (bf16_t)(w[r >> 1] >> (16 * (r & 1)));
@@ -338,25 +453,28 @@ int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
 // a group's part of the workspace
 int64_t group_bytes(const DphNsGroup& g, char* at, Group* out) {
   const int64_t m = g.rows < g.cols ? g.rows : g.cols, n = g.rows < g.cols ? g.cols : g.rows;
-  const int64_t mp = up64(m), np = up64(n), x = g.count * mp * np * 2, e = g.count * mp * mp * 2;
+  const int64_t mp = up64(m), np = up64(n), y = g.count * np * mp * 2, e = g.count * mp * mp * 2;
   const int64_t part = g.count * NS_PARTS * (int64_t)sizeof(double);
   const bool split = m <= NS_SPLIT;
   if (out) {
     out->part = reinterpret_cast<double*>(at);
     at += part;
-    out->xh = at;
-    out->xl = at + x;
-    out->xt[0] = at + 2 * x;
-    out->xt[1] = at + 3 * x;
-    out->e = at + 4 * x;
-    out->f = at + 4 * x + e;
-    at += 4 * x + 2 * e;
-    out->xtl[0] = split ? at : nullptr;
-    out->xtl[1] = split ? at + x : nullptr;
-    out->el = split ? at + 2 * x : nullptr;
-    out->fl = split ? at + 2 * x + e : nullptr;
+    auto take = [&](bool want, int64_t bytes) -> char* {
+      char* p = want ? at : nullptr;
+      if (want) at += bytes;
+      return p;
+    };
+    out->y[0] = take(true, y);
+    out->y[1] = take(true, y);
+    out->e = take(true, e);
+    out->f = take(true, e);
+    out->lo = take(!split, y / 2);
+    out->yl[0] = take(split, y);
+    out->yl[1] = take(split, y);
+    out->el = take(split, e);
+    out->fl = take(split, e);
   }
-  return part + 4 * x + 2 * e + (split ? 2 * x + 2 * e : 0);
+  return part + 2 * y + 2 * e + (split ? 2 * y + 2 * e : y / 2);
 }
 
 int check_groups(const DphNsGroup* groups, int64_t n, const char* who) {
@@ -389,21 +507,48 @@ extern "C" int64_t dph_newton_schulz_workspace(const DphNsGroup* groups, int64_t
 namespace dph {
 namespace {
 
-using NsTile = mt::Tile<128, 128, 2, 2>;
-
-template <int KIND>
-int launch_product(const Groups& gs0, const Step& st, hipStream_t stream) {
-  Groups gs = gs0;
+// the groups whose operands are split, or the others, and their tiles of C
+template <int KIND, bool SPLIT, class C>
+int64_t choose(const Groups& all, Groups* gs) {
   int64_t tiles = 0;
-  for (int i = 0; i < gs.ng; ++i) {
-    const Group& g = gs.g[i];
-    const int64_t tm = cdiv(g.m, NsTile::BM), tn = cdiv(g.n, NsTile::BN);
-    gs.first[i] = (int32_t)tiles;
+  gs->ng = 0;
+  for (int i = 0; i < all.ng; ++i) {
+    const Group& g = all.g[i];
+    if ((g.el != nullptr) != SPLIT) continue;
+    const int64_t tm = cdiv(g.m, C::BN), tn = cdiv(g.n, C::BM);
+    gs->first[gs->ng] = (int32_t)tiles;
+    gs->g[gs->ng++] = g;
     tiles += (KIND == GRAM || KIND == POLY ? tm * (tm + 1) / 2 : tm * tn) * g.cnt;
-    DPH_REQUIRE(tiles < (1 << 24), "dph_newton_schulz: too many tiles");
+    if (tiles >= (1 << 22)) return -1;
   }
-  hipLaunchKernelGGL((ns_product_kernel<KIND, NsTile>), dim3((unsigned)tiles), dim3(NsTile::NT), 0, stream, gs, st);
+  return tiles;
+}
+template <int KIND, bool SPLIT, class C>
+int launch_tiles(const Groups& all, const Step& st, hipStream_t stream) {
+  Groups gs = {};
+  const int64_t tiles = choose<KIND, SPLIT, C>(all, &gs);
+  DPH_REQUIRE(tiles >= 0, "dph_newton_schulz: too many tiles");
+  if (tiles == 0) return DPH_OK;
+  hipLaunchKernelGGL((ns_product_kernel<KIND, SPLIT, C>), dim3((unsigned)tiles), dim3(C::NT), 0, stream, gs, st);
   return check_launch("dph_newton_schulz");
+}
+
+// Tiles of 256 x 256 (one a CU), 128 x 128 or 64 x 64 (two): whichever needs least time by the rounds that its tiles take
+// on 256 CUs, a round of theirs counting 1, 0.58 and 0.27.  Measured, a whole call: 24 of 1024 x 4096 2.63 / 2.88 / 4.61
+// ms, 48 of 768 x 768 1.11 / 0.88 / 1.20 ms, one of 768 x 768 472 / 221 / 147 us, 8 of 448 x 768 396 / 188 / 152 us.
+template <int KIND>
+int launch_product(const Groups& gs, const Step& st, hipStream_t stream) {
+  using C256 = mt::Duo<256, 256, 1>;
+  using C128 = mt::Duo<128, 128, 2>;
+  using C64 = mt::Tile<64, 64, 2, 2, 4>;
+  DPH_TRY((launch_tiles<KIND, true, C64>(gs, st, stream)));
+  Groups some = {};
+  const int64_t t256 = choose<KIND, false, C256>(gs, &some), t128 = choose<KIND, false, C128>(gs, &some),
+                t64 = choose<KIND, false, C64>(gs, &some);
+  const double c256 = (double)cdiv(t256, 256), c128 = 0.58 * cdiv(t128, 512), c64 = 0.27 * cdiv(t64, 512);
+  if (t64 >= 0 && c64 < c128 && c64 < c256) return launch_tiles<KIND, false, C64>(gs, st, stream);
+  if (t128 >= 0 && c128 < c256) return launch_tiles<KIND, false, C128>(gs, st, stream);
+  return launch_tiles<KIND, false, C256>(gs, st, stream);
 }
 
 // up to NS_GROUPS groups, whose matrices start at mats
@@ -415,9 +560,9 @@ int run_groups(const DphNsMat* mats, const DphNsGroup* groups, int ng, int steps
   for (int i = 0; i < ng; ++i) {
     const DphNsGroup& in = groups[i];
     Group& g = gs.g[i];
-    g.trans = in.rows > in.cols;
-    g.m = (int32_t)(g.trans ? in.cols : in.rows);
-    g.n = (int32_t)(g.trans ? in.rows : in.cols);
+    g.wide = in.rows < in.cols;
+    g.m = (int32_t)(g.wide ? in.rows : in.cols);
+    g.n = (int32_t)(g.wide ? in.cols : in.rows);
     g.mp = (int32_t)up64(g.m);
     g.np = (int32_t)up64(g.n);
     g.cnt = (int32_t)in.count;
@@ -428,7 +573,7 @@ int run_groups(const DphNsMat* mats, const DphNsGroup* groups, int ng, int steps
     g.s = 1.f;
     while (g.s < 16384.f && (double)g.s * g.s * 64.0 <= (double)g.m * g.n) g.s *= 2.f;
     ws += group_bytes(in, ws, &g);
-    pg.g[i] = PackGroup{g.m, g.n, g.mp, g.np, g.in_f32, g.s, g.xh, g.xl, g.xt[0], g.xtl[0], g.part};
+    pg.g[i] = PackGroup{g.m, g.n, g.mp, g.np, g.in_f32, g.s, g.y[0], g.lo, g.yl[0], g.part};
   }
   // both packing passes, NS_MATS matrices at a time
   int gi = 0;
@@ -439,9 +584,9 @@ int run_groups(const DphNsMat* mats, const DphNsGroup* groups, int ng, int steps
     while (gi < ng && sum.n < NS_MATS) {
       const Group& g = gs.g[gi];
       const DphNsMat& in = mats[at++];
-      const int64_t rs = g.trans ? in.col_stride : in.row_stride, cs = g.trans ? in.row_stride : in.col_stride;
-      sum.m[sum.n++] = Mat{in.p, rs, cs, gi, (int32_t)idx, (int32_t)bs, 0};
-      pack.m[pack.n++] = Mat{in.p, rs, cs, gi, (int32_t)idx, (int32_t)bp, 0};
+      const int64_t ns = g.wide ? in.col_stride : in.row_stride, ms = g.wide ? in.row_stride : in.col_stride;
+      sum.m[sum.n++] = Mat{in.p, ns, ms, gi, (int32_t)idx, (int32_t)bs, 0};
+      pack.m[pack.n++] = Mat{in.p, ns, ms, gi, (int32_t)idx, (int32_t)bp, 0};
       bs += NS_PARTS;
       bp += (int64_t)(g.mp / 64) * (g.np / 64);
       DPH_REQUIRE(bp < (1 << 24), "dph_newton_schulz: too many tiles");

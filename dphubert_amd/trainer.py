@@ -341,9 +341,21 @@ class Trainer:
             self.reducer.finish()
             self.optimizer.launch()
 
+    WATCHDOG_QUIET_S = 0.35
+
+    def _quiet_watchdog(self):
+        """The process group's watchdog thread queries the events of eager collectives until it has seen them done (it
+        looks every 0.1 s).  A query that falls into a capture -- the collectives' stream is part of it -- is refused
+        ("operation not permitted on an event last recorded in a capturing stream") and ends the process, so a capture
+        starts after every collective is done and the watchdog has had three looks."""
+        if self.reducer.enabled and self.reducer.backend == "nccl":
+            torch.cuda.synchronize()
+            time.sleep(self.WATCHDOG_QUIET_S)
+
     def _capture(self, zero: bool, final: bool, prof=None):
         """Record one (micro-)step into a HIP graph (nothing executes during capture)."""
         from .kernels import LaunchProfiler
+        self._quiet_watchdog()
         ops.reset_zero_arena()           # zero-filled scratch must be allocated (and filled) inside the graph
         g = torch.cuda.CUDAGraph()
         try:
@@ -377,6 +389,7 @@ class Trainer:
         m = self.module
         side = m.teacher_stream
         from . import kernels as K
+        self._quiet_watchdog()
         ops.reset_zero_arena()
         try:
             if self._tgraph is None:

@@ -87,8 +87,7 @@ def test_workspace_is_refused_for_bad_groups():
     assert _lib.lib().dph_newton_schulz_workspace(g, 1) == -1
     assert _lib.lib().dph_newton_schulz_workspace(None, 1) == -1
     g[0].rows, g[0].cols, g[0].count = 70, 64, 2
-    # partial sums, X in two halves and two transposes of 64 x 128, E and F of 64 x 64; up to 128 rows the transposes, E and
-    # F have lower halves too
-    assert _lib.lib().dph_newton_schulz_workspace(g, 1) == 2 * (64 * 8 + 6 * 64 * 128 * 2 + 4 * 64 * 64 * 2)
+    # partial sums, Y twice (128 x 64), E and F of 64 x 64, the lower halves of all (up to 128 rows); above, 8 bits more of Y
+    assert _lib.lib().dph_newton_schulz_workspace(g, 1) == 2 * (64 * 8 + 4 * 64 * 128 * 2 + 4 * 64 * 64 * 2)
     g[0].rows, g[0].cols = 129, 200
-    assert _lib.lib().dph_newton_schulz_workspace(g, 1) == 2 * (64 * 8 + 4 * 192 * 256 * 2 + 2 * 192 * 192 * 2)
+    assert _lib.lib().dph_newton_schulz_workspace(g, 1) == 2 * (64 * 8 + 2 * 192 * 256 * 2 + 192 * 256 + 2 * 192 * 192 * 2)
