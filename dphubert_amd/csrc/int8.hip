@@ -6,8 +6,6 @@
 // quantised on the way in, a row at a time, either as they stand or as the output of a LayerNorm.
 #include "mfma_tile.h"
 
-#include <stdlib.h>
-
 #include <type_traits>
 
 namespace dph {
@@ -26,35 +24,54 @@ __device__ __forceinline__ int quant1(float x, float inv, float s) {
   return (int)t;
 }
 
+// 16 bytes at any alignment of the element (one load: the hardware takes it)
+__device__ __forceinline__ uint4 ld16(const void* p) {
+  uint4 r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+
+// 8 elements as they are in memory (bf16: 16 bytes, fp32: 32), zeros past K
 template <typename XT>
-__device__ __forceinline__ float ld1(const XT* p) {
-  if constexpr (std::is_same_v<XT, float>) return *p;
-  else return bf2f(*p);
-}
-
-// 8 consecutive elements, 16-byte aligned
-__device__ __forceinline__ void ld8v(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void ld8v(const bf16_t* p, float (&v)[8]) {
-  const uint4 r = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+struct Raw8 {
+  uint4 a, b;   // (b: fp32 only)
+  __device__ __forceinline__ void load(const XT* row, int c, int K) {
+    constexpr bool F = std::is_same_v<XT, float>;
+    if (c + 8 <= K) {
+      a = ld16(row + c);
+      if constexpr (F) b = ld16(row + c + 4);
+    } else {
+      uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < 8; ++i) {
+        w[i] = 0;
+        if (c + i < K) {
+          if constexpr (F) w[i] = __float_as_uint(row[c + i]);
+          else w[i] = row[c + i];
+        }
+      }
+      if constexpr (F) {
+        a = make_uint4(w[0], w[1], w[2], w[3]);
+        b = make_uint4(w[4], w[5], w[6], w[7]);
+      } else {
+        a = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+      }
+    }
   }
-}
-
-template <bool VEC, typename XT>
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (std::is_same_v<XT, float>) v[i] = __uint_as_float(w[i]);
+      else v[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    }
+  }
+};
+template <typename XT>
 __device__ __forceinline__ void load8(const XT* row, int c, int K, float (&v)[8]) {
-  if (VEC && c + 8 <= K) {
-    ld8v(row + c, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? ld1(row + c + i) : 0.f;
-  }
+  Raw8<XT> r;
+  r.load(row, c, K);
+  r.get(v);
 }
 
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
@@ -75,9 +92,24 @@ __device__ __forceinline__ uint2 pack8(const float (&v)[8], float inv, float s) 
   return make_uint2(w[0], w[1]);
 }
 
-// One wave a row: the largest |x|, then the integers (the row's second reading comes from the L2).  ldq is a multiple
-// of 16 and the row's bytes from K on are written as zeros.
-template <typename XT, bool VEC>
+// exact-erf GELU as common.h's (Abramowitz & Stegun 7.1.26, 1.5e-7), in the form max(x, 0) - |x| erfc(|x| / sqrt 2) / 2: no
+// comparison, and the halves and square roots are in the constants (58 -> 56 us at 7984 x 4096 x 1024, where it is a third)
+__device__ __forceinline__ float gelu_i8(float x) {
+  const float ax = fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.23164189f, ax, 1.0f));
+  const float p = t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+  return fmaf(-ax, p * __builtin_amdgcn_exp2f(x * x * -0.72134752f), fmaxf(x, 0.f));
+}
+
+__device__ __forceinline__ uint32_t umax8(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+
+// One wave a row, read once: NV chunks of 8 elements a lane stay in registers (NV 512 columns); longer rows are read
+// again for their integers (NV = 0).  ldq is a multiple of 16; the row's bytes from K on are written as zeros.
+template <typename XT, int NV>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const XT* __restrict__ x, int64_t rows, int32_t K, int64_t ldx,
                                                          int8_t* __restrict__ q, int64_t ldq,
                                                          float* __restrict__ scale) {
@@ -85,41 +117,50 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const XT* __restrict__ 
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
   const XT* xr = x + r * ldx;
-  uint32_t m = 0;
-  for (int c = lane * 8; c < K; c += 512) {
-    float v[8];
-    load8<VEC>(xr, c, K, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  }
-  const float s = row_scale(wave_umax(m));
-  const bool ok = s == s;
-  const float inv = 1.0f / s;
   int8_t* qr = q + r * ldq;
-  for (int c = lane * 8; c < ldq; c += 512) {
-    float v[8];
-    load8<VEC>(xr, c, K, v);
-    *reinterpret_cast<uint2*>(qr + c) = ok ? pack8(v, inv, s) : make_uint2(0, 0);
+  float v[8];
+  uint32_t m = 0;
+  if constexpr (NV > 0) {
+    Raw8<XT> raw[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) raw[j].load(xr, j * 512 + lane * 8, K);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      raw[j].get(v);
+      m = max(m, umax8(v));
+    }
+    const float s = row_scale(wave_umax(m)), inv = 1.0f / s;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = j * 512 + lane * 8;
+      raw[j].get(v);
+      if (c < ldq) *reinterpret_cast<uint2*>(qr + c) = s == s ? pack8(v, inv, s) : make_uint2(0, 0);
+    }
+    if (lane == 0) scale[r] = s;
+  } else {
+    for (int c = lane * 8; c < K; c += 512) {
+      load8(xr, c, K, v);
+      m = max(m, umax8(v));
+    }
+    const float s = row_scale(wave_umax(m)), inv = 1.0f / s;
+    for (int c = lane * 8; c < ldq; c += 512) {
+      load8(xr, c, K, v);
+      *reinterpret_cast<uint2*>(qr + c) = s == s ? pack8(v, inv, s) : make_uint2(0, 0);
+    }
+    if (lane == 0) scale[r] = s;
   }
-  if (lane == 0) scale[r] = s;
 }
 
-// LayerNorm of a row (fp32 two-pass statistics) quantised from its fp32 values, and the values themselves in bf16 where
-// the residual branch wants them.  One wave a row; rows of up to 2048 columns stay in registers (NV chunks of 8 a lane).
-template <typename XT, bool VEC, int NV>
-__global__ void __launch_bounds__(256) ln_quant_kernel(const XT* __restrict__ x, const float* __restrict__ gamma,
-                                                       const float* __restrict__ beta, int64_t rows, int32_t K,
-                                                       int64_t ldx, float eps, bf16_t* __restrict__ y, int64_t ldy,
-                                                       int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  const XT* xr = x + r * ldx;
-  float v[NV][8];
+// LayerNorm of a row (fp32 two-pass statistics) into v; the values go to yr in bf16 too where the residual branch wants
+// them.  One wave; NV chunks of 8 columns a lane.  Returns the largest |v| as bits.
+template <int NV, typename XT>
+__device__ __forceinline__ uint32_t norm_row(const XT* xr, const float* __restrict__ gamma,
+                                             const float* __restrict__ beta, int K, float eps, bf16_t* yr, bool yvec,
+                                             int lane, float (&v)[NV][8]) {
   float sum = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    load8<VEC>(xr, j * 512 + lane * 8, K, v[j]);
+    load8(xr, j * 512 + lane * 8, K, v[j]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += v[j][i];
   }
@@ -138,33 +179,41 @@ __global__ void __launch_bounds__(256) ln_quant_kernel(const XT* __restrict__ x,
   for (int j = 0; j < NV; ++j) {
     const int c = j * 512 + lane * 8;
     float g[8], b[8];
-    load8<VEC>(gamma, c, K, g);
-    load8<VEC>(beta, c, K, b);
+    load8(gamma, c, K, g);
+    load8(beta, c, K, b);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[j][i] = c + i < K ? (v[j][i] - mean) * rstd * g[i] + b[i] : 0.f;
-      m = max(m, __float_as_uint(v[j][i]) & 0x7fffffffu);
-    }
-    if (y) {
-      bf16_t* yr = y + r * ldy + c;
-      if (VEC && c + 8 <= K) {
-        *reinterpret_cast<uint4*>(yr) = make_uint4(pack2bf(v[j][0], v[j][1]), pack2bf(v[j][2], v[j][3]),
-                                                   pack2bf(v[j][4], v[j][5]), pack2bf(v[j][6], v[j][7]));
+    for (int i = 0; i < 8; ++i) v[j][i] = c + i < K ? (v[j][i] - mean) * rstd * g[i] + b[i] : 0.f;
+    m = max(m, umax8(v[j]));
+    if (yr) {
+      if (yvec && c + 8 <= K) {
+        *reinterpret_cast<uint4*>(yr + c) = make_uint4(pack2bf(v[j][0], v[j][1]), pack2bf(v[j][2], v[j][3]),
+                                                       pack2bf(v[j][4], v[j][5]), pack2bf(v[j][6], v[j][7]));
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (c + i < K) yr[i] = f2bf(v[j][i]);
+          if (c + i < K) yr[c + i] = f2bf(v[j][i]);
       }
     }
   }
-  const float s = row_scale(wave_umax(m));
-  const bool ok = s == s;
+  return wave_umax(m);
+}
+
+template <typename XT, int NV>
+__global__ void __launch_bounds__(256) ln_quant_kernel(const XT* __restrict__ x, const float* __restrict__ gamma,
+                                                       const float* __restrict__ beta, int64_t rows, int32_t K,
+                                                       int64_t ldx, float eps, bf16_t* __restrict__ y, int64_t ldy,
+                                                       bool yvec, int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  float v[NV][8];
+  const float s = row_scale(norm_row<NV>(x + r * ldx, gamma, beta, K, eps, y ? y + r * ldy : nullptr, yvec, lane, v));
   const float inv = 1.0f / s;
   int8_t* qr = q + r * ldq;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = j * 512 + lane * 8;
-    if (c < ldq) *reinterpret_cast<uint2*>(qr + c) = ok ? pack8(v[j], inv, s) : make_uint2(0, 0);
+    if (c < ldq) *reinterpret_cast<uint2*>(qr + c) = s == s ? pack8(v[j], inv, s) : make_uint2(0, 0);
   }
   if (lane == 0) scale[r] = s;
 }
@@ -178,80 +227,131 @@ struct LinearI8 {
   void* out;
   int64_t ldr, ldo;
   int32_t ntn, ntiles;
-  int32_t vec;      // 4 consecutive columns of res and out are one aligned access
+  int32_t vec;   // rows of res and out are 16-byte aligned
 };
 
-// RES: 0 none, 1 bf16, 2 fp32 (the output has the residual's type; without one it is bf16, or fp32 with OUT32)
-template <class C, bool GELU, int RES, bool OUT32>
-__device__ __forceinline__ void store_tile(const LinearI8& a, const mt::i32x4_t (&acc)[C::FM][C::FN], int mw, int nw,
-                                           int lane) {
-  const int ml = mw + (lane & 15), nl = nw + 4 * (lane >> 4);
-  float ws[C::FN][4], bias[C::FN][4];
+// W consecutive columns of the residual's row m from n on, as they are in memory (zeros past N).  RES: 0 none, 1 bf16, 2 fp32
+template <int W, int RES>
+struct Resid {
+  uint32_t w[RES == 2 ? W : W / 2];
+  __device__ __forceinline__ void load(const LinearI8& a, int64_t m, int n) {
+    const int64_t o = m * a.ldr + n;
+    if constexpr (RES == 1) {
+      const bf16_t* p = reinterpret_cast<const bf16_t*>(a.res) + o;
+      if (a.vec && n + W <= a.N) {
+        const uint4 r = *reinterpret_cast<const uint4*>(p);
+        w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+      } else {
 #pragma unroll
-  for (int j = 0; j < C::FN; ++j)
+        for (int c = 0; c < W; c += 2)
+          w[c / 2] = (n + c < a.N ? (uint32_t)p[c] : 0u) | (n + c + 1 < a.N ? (uint32_t)p[c + 1] << 16 : 0u);
+      }
+    } else if constexpr (RES == 2) {
+      const float* p = reinterpret_cast<const float*>(a.res) + o;
+      if (a.vec && n + W <= a.N) {
+        const uint4 r = *reinterpret_cast<const uint4*>(p);
+        w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+      } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int n = min(nl + 16 * j + r, a.N - 1);
-      ws[j][r] = a.ws[n];
-      bias[j][r] = a.bias ? a.bias[n] : 0.f;
+        for (int c = 0; c < W; ++c) w[c] = n + c < a.N ? __float_as_uint(p[c]) : 0u;
+      }
     }
+  }
+  __device__ __forceinline__ float get(int c) const {
+    if constexpr (RES == 0) return 0.f;
+    if constexpr (RES == 2) return __uint_as_float(w[c]);
+    return __uint_as_float(c & 1 ? w[c / 2] & 0xffff0000u : w[c / 2] << 16);
+  }
+};
+
+// The row's W sums v, finished and stored (the output has the residual's type; without one it is bf16, or fp32 with OUT32)
+template <int W, bool GELU, int RES, bool OUT32>
+__device__ __forceinline__ void finish(const LinearI8& a, int64_t m, int n, float xs, const float* ws, const float* bias,
+                                       const Resid<W, RES>& t, float* v) {
+  static_assert(W == (OUT32 ? 4 : 8), "16 bytes");
+  const int64_t o = m * a.ldo + n;
+#pragma unroll
+  for (int c = 0; c < W; ++c) {
+    v[c] = fmaf(v[c] * xs, ws[c], bias[c]);
+    if (GELU) v[c] = gelu_i8(v[c]);
+    if constexpr (RES != 0) v[c] += t.get(c);
+  }
+  const bool vec = a.vec && n + W <= a.N;
+  if constexpr (OUT32) {
+    float* p = reinterpret_cast<float*>(a.out) + o;
+    if (vec) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < W; ++c)
+        if (n + c < a.N) p[c] = v[c];
+    }
+  } else {
+    bf16_t* p = reinterpret_cast<bf16_t*>(a.out) + o;
+    if (vec) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+    } else {
+#pragma unroll
+      for (int c = 0; c < W; ++c)
+        if (n + c < a.N) p[c] = f2bf(v[c]);
+    }
+  }
+}
+
+// A tile's scales and biases: asked for before the product, in the LDS after it (read from memory between the stores they
+// cost a latency a fragment row: the stores might write them, for all the compiler knows)
+template <class C>
+struct Scales {
+  float xs[C::BM], ws[C::BN], bias[C::BN];
+};
+template <class C>
+struct ScaleRegs {
+  static_assert(C::NT >= C::BM && C::NT >= C::BN, "one of each a thread");
+  float xs, ws, bias;
+  __device__ __forceinline__ void load(const LinearI8& a, int m0, int n0) {
+    const int t = threadIdx.x, n = min(n0 + t, a.N - 1);
+    if (t < C::BM) xs = a.xs[min(m0 + t, a.M - 1)];
+    if (t < C::BN) {
+      ws = a.ws[n];
+      bias = a.bias ? a.bias[n] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(Scales<C>& s) const {
+    const int t = threadIdx.x;
+    if (t < C::BM) s.xs[t] = xs;
+    if (t < C::BN) s.ws[t] = ws, s.bias[t] = bias;
+    __syncthreads();
+  }
+};
+
+template <class C, bool GELU, int RES, bool OUT32>
+__device__ __forceinline__ void store_tile(const LinearI8& a, const mt::i32x4_t (&acc)[C::FM][C::FN],
+                                           const Scales<C>& sc, int m0, int n0, int wave, int lane) {
+  using V = mt::Strip<C::FN, OUT32 ? 4 : 8>;
+  const int mt0 = wave / C::WC * C::WTM + (lane & 15), nt0 = wave % C::WC * C::WTN;
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
-    const int m = ml + 16 * i;
-    if (m >= a.M) continue;
-    const float xs = a.xs[m];
+    const int mt = mt0 + 16 * i, m = m0 + mt;
+    // (a fragment row's residual just before its stores: with two or more rows asked for ahead, reads and writes come in
+    // bursts, 107 against 99 us at 7984 x 4096 x 1024 in fp32)
+    Resid<V::W, RES> t[V::NG];
 #pragma unroll
-    for (int j = 0; j < C::FN; ++j) {
-      const int n = nl + 16 * j;
-      if (n >= a.N) continue;
-      const int64_t o = (int64_t)m * a.ldo + n, ro = (int64_t)m * a.ldr + n;
-      const bool vec = a.vec && n + 4 <= a.N;
-      float v[4];
+    for (int q = 0; q < V::NG; ++q) {
+      const int n = n0 + nt0 + V::col(q, lane);
+      if (RES != 0 && m < a.M && n < a.N) t[q].load(a, m, n);
+    }
+    uint32_t b[4 * C::FN];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        v[r] = fmaf((float)acc[i][j][r] * xs, ws[j][r], bias[j][r]);
-        if (GELU) v[r] = gelu_f(v[r]);
-      }
-      if constexpr (RES == 1) {
-        const bf16_t* p = reinterpret_cast<const bf16_t*>(a.res) + ro;
-        if (vec) {
-          float t[4];
-          ring::unpack_bf16x4(*reinterpret_cast<const uint2*>(p), t);
+    for (int r = 0; r < 4 * C::FN; ++r) b[r] = (uint32_t)acc[i][r >> 2][r & 3];
+    V::exchange(b);
+    const float xs = sc.xs[mt];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] += t[r];
-        } else {
+    for (int q = 0; q < V::NG; ++q) {
+      const int nt = nt0 + V::col(q, lane), n = n0 + nt;
+      float v[V::W];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] += n + r < a.N ? bf2f(p[r]) : 0.f;
-        }
-      } else if constexpr (RES == 2) {
-        const float* p = reinterpret_cast<const float*>(a.res) + ro;
-        if (vec) {
-          const float4 t = *reinterpret_cast<const float4*>(p);
-          v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] += n + r < a.N ? p[r] : 0.f;
-        }
-      }
-      if constexpr (OUT32) {
-        float* p = reinterpret_cast<float*>(a.out) + o;
-        if (vec) {
-          *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n + r < a.N) p[r] = v[r];
-        }
-      } else {
-        bf16_t* p = reinterpret_cast<bf16_t*>(a.out) + o;
-        if (vec) {
-          *reinterpret_cast<uint2*>(p) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n + r < a.N) p[r] = f2bf(v[r]);
-        }
-      }
+      for (int r = 0; r < V::W; ++r) v[r] = (float)(int32_t)b[V::W * q + r];
+      if (m < a.M && n < a.N) finish<V::W, GELU, RES, OUT32>(a, m, n, xs, sc.ws + nt, sc.bias + nt, t[q], v);
     }
   }
 }
@@ -266,58 +366,189 @@ __global__ void __launch_bounds__(C::NT, C::WPE) linear_i8_kernel(const LinearI8
   const int first = t / per * GM, h = min(GM, ntm - first), l = t % per;
   const int m0 = (first + l % h) * C::BM, n0 = l / h * C::BN;
   mt::i32x4_t acc[C::FM][C::FN];
-  mt::product_of<mt::I8, C>(a.x, a.w, a.K, m0, n0, acc, smem, wave, lane, [&]() { mt::clear<mt::I8, C>(acc); });
-  store_tile<C, GELU, RES, OUT32>(a, acc, m0 + wave / C::WC * C::WTM, n0 + wave % C::WC * C::WTN, lane);
+  ScaleRegs<C> sr;
+  mt::product_of<mt::I8, C>(a.x, a.w, a.K, m0, n0, acc, smem, wave, lane, [&]() {
+    sr.load(a, m0, n0);
+    mt::clear<mt::I8, C>(acc);
+  });
+  Scales<C>& sc = *reinterpret_cast<Scales<C>*>(smem);    // (the product is through with its images)
+  sr.store(sc);
+  store_tile<C, GELU, RES, OUT32>(a, acc, sc, m0, n0, wave, lane);
+}
+
+// Up to 16 rows of x in one launch: a workgroup quantises all of them for itself (they come from the L2), into the LDS,
+// and multiplies 16 channels of W, read once and straight into the registers, a quarter of K a wave.  What bounds it is
+// the latency of one read of W.
+struct SmallI8 {
+  LinearI8 l;
+  const void* x;
+  int64_t ldx;
+  const float *gamma, *beta;
+  bf16_t* norm;
+  int64_t ldn;
+  float eps;
+  int32_t yvec;        // rows of norm are 16-byte aligned
+  int32_t lds_ld;      // bytes of a row of q in the LDS
+};
+
+template <typename XT, int NV>
+__device__ __forceinline__ float small_quant(const SmallI8& a, int r, int8_t* qr, int lane) {
+  const int K = a.l.K;
+  const XT* xr = reinterpret_cast<const XT*>(a.x) + r * a.ldx;
+  float s;
+  if constexpr (NV > 0) {       // LayerNorm
+    float v[NV][8];
+    bf16_t* yr = a.norm && blockIdx.x == 0 ? a.norm + r * a.ldn : nullptr;
+    s = row_scale(norm_row<NV>(xr, a.gamma, a.beta, K, a.eps, yr, a.yvec, lane, v));
+    const float inv = 1.0f / s;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = j * 512 + lane * 8;
+      if (c < a.lds_ld) *reinterpret_cast<uint2*>(qr + c) = s == s ? pack8(v[j], inv, s) : make_uint2(0, 0);
+    }
+  } else {
+    uint32_t m = 0;
+    float v[8];
+    for (int c = lane * 8; c < K; c += 512) {
+      load8(xr, c, K, v);
+      m = max(m, umax8(v));
+    }
+    s = row_scale(wave_umax(m));
+    const float inv = 1.0f / s;
+    for (int c = lane * 8; c < a.lds_ld; c += 512) {
+      load8(xr, c, K, v);
+      *reinterpret_cast<uint2*>(qr + c) = s == s ? pack8(v, inv, s) : make_uint2(0, 0);
+    }
+  }
+  return s;
+}
+
+constexpr int SMALL_M = 16, SMALL_LDS = 56 * 1024;   // (static and dynamic LDS within 64 KB)
+// bytes of a row of q in the LDS: whole steps of 64, and 16 more so that the rows start on different banks
+constexpr int64_t small_ld(int64_t K) { return ((K + 63) & ~(int64_t)63) + 16; }
+
+template <typename XT, int NV, bool GELU, int RES, bool OUT32>
+__global__ void __launch_bounds__(256) small_i8_kernel(const SmallI8 a) {
+  extern __shared__ __align__(16) char sq[];     // [M][lds_ld] integers
+  __shared__ float scale[SMALL_M];
+  __shared__ int32_t part[4][SMALL_M][17];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int M = a.l.M, n0 = blockIdx.x * 16;
+  // W's first chunks are asked for before x is looked at
+  const int steps = (a.l.K + 63) >> 6, per = (steps + 3) >> 2, k0 = wave * per, k1 = min(steps, k0 + per);
+  const int kend = (a.l.K + 15) & ~15;
+  const char* wr = a.l.w.p + (int64_t)min(n0 + (lane & 15), a.l.N - 1) * a.l.w.ld;
+  auto ldw = [&](int k) {
+    const int off = k * 64 + (lane >> 4) * 16;
+    return *reinterpret_cast<const mt::i32x4_t*>(wr + (off < kend ? off : 0));
+  };
+  constexpr int AHEAD = 4;
+  mt::i32x4_t w[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (k0 + i < k1) w[i] = ldw(k0 + i);
+  for (int r = wave; r < M; r += 4) {
+    const float s = small_quant<XT, NV>(a, r, reinterpret_cast<int8_t*>(sq) + r * a.lds_ld, lane);
+    if (lane == 0) scale[r] = s;
+  }
+  __syncthreads();
+  // (rows past M: the last one's, never stored; chunks past K are zeros in the LDS)
+  const char* qr = sq + min(lane & 15, M - 1) * a.lds_ld + (lane >> 4) * 16;
+  mt::i32x4_t acc = {0, 0, 0, 0};
+  for (int k = k0; k < k1; k += AHEAD) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (k + i >= k1) break;
+      const mt::i32x4_t now = w[i];
+      if (k + i + AHEAD < k1) w[i] = ldw(k + i + AHEAD);
+      acc = mt::I8::mfma(now, *reinterpret_cast<const mt::i32x4_t*>(qr + (k + i) * 64), acc);
+    }
+  }
+  // acc: channel n0 + 4 (lane / 16) + r of row lane % 16
+#pragma unroll
+  for (int r = 0; r < 4; ++r) part[wave][lane & 15][4 * (lane >> 4) + r] = acc[r];
+  __syncthreads();
+  const int m = threadIdx.x >> 4, c = threadIdx.x & 15, n = n0 + c;
+  if (m < M && n < a.l.N) {
+    float v = (float)(part[0][m][c] + part[1][m][c] + part[2][m][c] + part[3][m][c]);
+    v = fmaf(v * scale[m], a.l.ws[n], a.l.bias ? a.l.bias[n] : 0.f);
+    if (GELU) v = gelu_i8(v);
+    if constexpr (RES == 1) v += bf2f(reinterpret_cast<const bf16_t*>(a.l.res)[m * a.l.ldr + n]);
+    if constexpr (RES == 2) v += reinterpret_cast<const float*>(a.l.res)[m * a.l.ldr + n];
+    if constexpr (OUT32) reinterpret_cast<float*>(a.l.out)[m * a.l.ldo + n] = v;
+    else reinterpret_cast<bf16_t*>(a.l.out)[m * a.l.ldo + n] = f2bf(v);
+  }
+}
+
+template <typename F>
+void with_epilogue(bool gelu, int res, bool out32, F f) {
+  auto go = [&](auto g) {
+    using std::integral_constant;
+    if (res == 1) f(g, integral_constant<int, 1>{}, std::false_type{});
+    else if (res == 2) f(g, integral_constant<int, 2>{}, std::true_type{});
+    else if (out32) f(g, integral_constant<int, 0>{}, std::true_type{});
+    else f(g, integral_constant<int, 0>{}, std::false_type{});
+  };
+  if (gelu) go(std::true_type{});
+  else go(std::false_type{});
 }
 
 template <class C>
 void launch_linear(const LinearI8& a, bool gelu, int res, bool out32, hipStream_t stream) {
-  const dim3 g((unsigned)a.ntiles), b(C::NT);
-#define DPH_LIN(G, R, O) hipLaunchKernelGGL((linear_i8_kernel<C, G, R, O>), g, b, 0, stream, a)
-  if (gelu) {
-    if (res == 1) DPH_LIN(true, 1, false);
-    else if (res == 2) DPH_LIN(true, 2, true);
-    else if (out32) DPH_LIN(true, 0, true);
-    else DPH_LIN(true, 0, false);
-  } else {
-    if (res == 1) DPH_LIN(false, 1, false);
-    else if (res == 2) DPH_LIN(false, 2, true);
-    else if (out32) DPH_LIN(false, 0, true);
-    else DPH_LIN(false, 0, false);
-  }
-#undef DPH_LIN
+  with_epilogue(gelu, res, out32, [&](auto g, auto r, auto o) {
+    hipLaunchKernelGGL((linear_i8_kernel<C, decltype(g)::value, decltype(r)::value, decltype(o)::value>),
+                       dim3((unsigned)a.ntiles), dim3(C::NT), 0, stream, a);
+  });
+}
+
+// f(chunks of 512 columns in the registers)
+template <typename F>
+void with_chunks(int64_t K, F f) {
+  if (K <= 512) f(std::integral_constant<int, 1>{});
+  else if (K <= 1024) f(std::integral_constant<int, 2>{});
+  else f(std::integral_constant<int, 4>{});
+}
+
+template <typename XT>
+void launch_small(const SmallI8& a, bool gelu, int res, bool out32, hipStream_t stream) {
+  const dim3 g((unsigned)cdiv(a.l.N, 16));
+  const size_t lds = (size_t)a.l.M * a.lds_ld;
+  with_epilogue(gelu, res, out32, [&](auto ge, auto re, auto o) {
+    auto go = [&](auto nv) {
+      hipLaunchKernelGGL((small_i8_kernel<XT, decltype(nv)::value, decltype(ge)::value, decltype(re)::value,
+                                          decltype(o)::value>),
+                         g, dim3(256), lds, stream, a);
+    };
+    if (a.gamma) {
+      if constexpr (decltype(re)::value == 0 && !decltype(o)::value) with_chunks(a.l.K, go);
+    } else {
+      go(std::integral_constant<int, 0>{});
+    }
+  });
 }
 
 template <typename XT>
 int quant_rows(const void* x, int64_t rows, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                hipStream_t stream) {
-  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * sizeof(XT) % 16 == 0;
-  const dim3 g((unsigned)cdiv(rows, 4));
-  const XT* xp = reinterpret_cast<const XT*>(x);
-  if (vec) hipLaunchKernelGGL((quant_rows_kernel<XT, true>), g, dim3(256), 0, stream, xp, rows, (int32_t)K, ldx, q, ldq, scale);
-  else hipLaunchKernelGGL((quant_rows_kernel<XT, false>), g, dim3(256), 0, stream, xp, rows, (int32_t)K, ldx, q, ldq, scale);
+  auto go = [&](auto nv) {
+    hipLaunchKernelGGL((quant_rows_kernel<XT, decltype(nv)::value>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, stream,
+                       reinterpret_cast<const XT*>(x), rows, (int32_t)K, ldx, q, ldq, scale);
+  };
+  if (ldq <= 2048) with_chunks(ldq, go);
+  else if (ldq <= 4096) go(std::integral_constant<int, 8>{});
+  else go(std::integral_constant<int, 0>{});
   return check_launch("dph_quant_rows_i8");
 }
 
+bool norm_vec(const DphLinearI8Args& a) { return reinterpret_cast<uintptr_t>(a.norm_out) % 16 == 0 && a.ld_norm % 8 == 0; }
+
 template <typename XT>
 int ln_quant(const DphLinearI8Args& a, hipStream_t stream) {
-  const uintptr_t al = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.ln_weight) |
-                       reinterpret_cast<uintptr_t>(a.ln_bias) | reinterpret_cast<uintptr_t>(a.norm_out) |
-                       (uintptr_t)(a.ldx * sizeof(XT)) | (uintptr_t)(a.norm_out ? a.ld_norm * 2 : 0);
-  const bool vec = al % 16 == 0;
-  const dim3 g((unsigned)cdiv(a.M, 4));
-  auto go = [&](auto vc, auto nv) {
-    hipLaunchKernelGGL((ln_quant_kernel<XT, decltype(vc)::value, decltype(nv)::value>), g, dim3(256), 0, stream,
+  with_chunks(a.K, [&](auto nv) {
+    hipLaunchKernelGGL((ln_quant_kernel<XT, decltype(nv)::value>), dim3((unsigned)cdiv(a.M, 4)), dim3(256), 0, stream,
                        reinterpret_cast<const XT*>(a.x), a.ln_weight, a.ln_bias, a.M, (int32_t)a.K, a.ldx, a.ln_eps,
-                       reinterpret_cast<bf16_t*>(a.norm_out), a.ld_norm, a.q, a.ldq, a.q_scale);
-  };
-  auto nvs = [&](auto vc) {
-    if (a.K <= 512) go(vc, std::integral_constant<int, 1>{});
-    else if (a.K <= 1024) go(vc, std::integral_constant<int, 2>{});
-    else go(vc, std::integral_constant<int, 4>{});
-  };
-  if (vec) nvs(std::true_type{});
-  else nvs(std::false_type{});
+                       reinterpret_cast<bf16_t*>(a.norm_out), a.ld_norm, norm_vec(a), a.q, a.ldq, a.q_scale);
+  });
   return check_launch("dph_linear_i8 (LayerNorm)");
 }
 
@@ -343,6 +574,18 @@ extern "C" int dph_quant_rows_i8(const void* x, int x_f32, int64_t rows, int64_t
                : quant_rows<bf16_t>(x, rows, K, ldx, q, ldq, scale, stream);
 }
 
+// whether x (given, not its integers) goes through the kernel of up to 16 rows, which needs no q
+static bool small_i8(const DphLinearI8Args& a) {
+  return a.x && a.M <= SMALL_M && a.M * small_ld(a.K) <= SMALL_LDS && a.N > 0;
+}
+
+extern "C" int64_t dph_linear_i8_workspace(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N < 0 || K <= 0) return 0;
+  DphLinearI8Args a = {};
+  a.M = M, a.N = N, a.K = K, a.x = &a;
+  return small_i8(a) ? 0 : M * (((K + 15) & ~(int64_t)15) + 4);
+}
+
 extern "C" int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream) {
   DPH_REQUIRE(args, "dph_linear_i8: null args");
   const DphLinearI8Args& a = *args;
@@ -350,22 +593,32 @@ extern "C" int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream) {
   DPH_REQUIRE(a.M <= ROWS_MAX && a.N <= ROWS_MAX && a.K <= DPH_I8_K_MAX,
               "dph_linear_i8: M and N up to 2^25, K up to %d (32-bit sums)", DPH_I8_K_MAX);
   if (a.M == 0) return DPH_OK;
-  DPH_REQUIRE(a.q && a.q_scale, "dph_linear_i8: null operand");
-  DPH_REQUIRE(a.ldq >= a.K && a.ldq % 16 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0,
-              "dph_linear_i8: rows of q start 16 bytes apart or a multiple of it");
   DPH_REQUIRE(a.act == DPH_ACT_NONE || a.act == DPH_ACT_GELU, "dph_linear_i8: act is none or gelu");
   const bool out32 = a.out_dtype == DPH_OUT_F32;
   DPH_REQUIRE(out32 || a.out_dtype == DPH_OUT_BF16, "dph_linear_i8: out is bf16 or fp32");
   DPH_REQUIRE(!a.residual || (a.residual_f32 != 0) == out32, "dph_linear_i8: out has the residual's type");
+  DPH_REQUIRE(!a.residual || a.ldr >= a.N || a.M == 1, "dph_linear_i8: rows of the residual overlap");
+  const bool small = small_i8(a);
+  if (!small) {
+    DPH_REQUIRE(a.q && a.q_scale, "dph_linear_i8: null operand");
+    DPH_REQUIRE(a.ldq >= a.K && a.ldq % 16 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0,
+                "dph_linear_i8: rows of q start 16 bytes apart or a multiple of it");
+  }
   if (a.x) {
     DPH_REQUIRE(a.ldx >= a.K || a.M == 1, "dph_linear_i8: rows of x overlap");
     if (a.ln_weight) {
       DPH_REQUIRE(a.ln_bias, "dph_linear_i8: LayerNorm without a bias");
       DPH_REQUIRE(a.K <= DPH_I8_LN_MAX, "dph_linear_i8: LayerNorm of up to %d columns", DPH_I8_LN_MAX);
-      DPH_REQUIRE(a.ldq <= (a.K <= 512 ? 512 : a.K <= 1024 ? 1024 : 2048), "dph_linear_i8: ldq of the LayerNorm form");
-      DPH_TRY(a.x_f32 ? ln_quant<float>(a, stream) : ln_quant<bf16_t>(a, stream));
-    } else {
-      DPH_TRY(dph_quant_rows_i8(a.x, a.x_f32, a.M, a.K, a.ldx, a.q, a.ldq, a.q_scale, stream));
+      DPH_REQUIRE(!a.norm_out || a.ld_norm >= a.K, "dph_linear_i8: rows of norm_out overlap");
+      DPH_REQUIRE(!a.residual && !out32, "dph_linear_i8: the LayerNorm form gives bf16 without a residual");
+    }
+    if (!small) {
+      if (a.ln_weight) {
+        DPH_REQUIRE(a.ldq <= (a.K <= 512 ? 512 : a.K <= 1024 ? 1024 : 2048), "dph_linear_i8: ldq of the LayerNorm form");
+        DPH_TRY(a.x_f32 ? ln_quant<float>(a, stream) : ln_quant<bf16_t>(a, stream));
+      } else {
+        DPH_TRY(dph_quant_rows_i8(a.x, a.x_f32, a.M, a.K, a.ldx, a.q, a.ldq, a.q_scale, stream));
+      }
     }
   }
   if (a.N == 0) return DPH_OK;
@@ -373,32 +626,40 @@ extern "C" int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream) {
   DPH_REQUIRE(a.ldw >= a.K && a.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0,
               "dph_linear_i8: rows of w start 16 bytes apart or a multiple of it");
   DPH_REQUIRE(a.ldo >= a.N || a.M == 1, "dph_linear_i8: rows of out overlap");
-  DPH_REQUIRE(a.ldq < (1 << 23) && a.ldw < (1 << 23), "dph_linear_i8: rows of q and w less than 2^23 bytes apart");
-  const int es = out32 ? 4 : 2;
+  DPH_REQUIRE((small || a.ldq < (1 << 23)) && a.ldw < (1 << 23),
+              "dph_linear_i8: rows of q and w less than 2^23 bytes apart");
+  const int es = out32 ? 4 : 2, res = a.residual ? (out32 ? 2 : 1) : 0;
   const uintptr_t al = reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.residual) |
                        (uintptr_t)(a.ldo * es) | (uintptr_t)(a.residual ? a.ldr * es : 0);
   LinearI8 p{{reinterpret_cast<const char*>(a.q), a.ldq, (int32_t)a.M},
              {reinterpret_cast<const char*>(a.w), a.ldw, (int32_t)a.N},
              (int32_t)a.M, (int32_t)a.N, (int32_t)a.K, a.q_scale, a.w_scale, a.bias, a.residual, a.out, a.ldr, a.ldo,
-             0, 0, al % (4 * es) == 0};
-  auto go = [&](auto c) -> int {
+             0, 0, al % 16 == 0};
+  const bool gelu = a.act == DPH_ACT_GELU;
+  if (small) {
+    SmallI8 sm{p, a.x, a.ldx, a.ln_weight, a.ln_bias, reinterpret_cast<bf16_t*>(a.norm_out), a.ld_norm, a.ln_eps,
+               norm_vec(a), (int32_t)small_ld(a.K)};
+    if (a.x_f32) launch_small<float>(sm, gelu, res, out32, stream);
+    else launch_small<bf16_t>(sm, gelu, res, out32, stream);
+    return check_launch("dph_linear_i8");
+  }
+  // Tiles of 256 x 256 (one a CU), 128 x 128 or 64 x 64 (two): whichever needs least time by the rounds that its tiles take
+  // on 256 CUs, a round of theirs counting 1, 0.55 and 0.27.  Measured, the product alone: 7984 x 1024 x 4096 62 / 45 / 66
+  // us, 8192 x 8192 x 8192 398 / 518 us / -, 7984 x 2304 x 768 32 / 24 / 36 us, 1497 x 768 x 1533 37 / 16 / 15 us.
+  using C256 = mt::Duo<256, 256, 1>;
+  using C128 = mt::Duo<128, 128, 2>;
+  using C64 = mt::Tile<64, 64, 2, 2, 4>;
+  auto tiles = [&](int b) { return cdiv(a.M, b) * cdiv(a.N, b); };
+  const double c256 = (double)cdiv(tiles(256), 256), c128 = 0.55 * cdiv(tiles(128), 512), c64 = 0.27 * cdiv(tiles(64), 512);
+  DPH_REQUIRE(tiles(256) < (1 << 22), "dph_linear_i8: too many tiles");
+  auto go = [&](auto c) {
     using C = decltype(c);
-    const int64_t ntm = cdiv(a.M, C::BM), ntn = cdiv(a.N, C::BN);
-    DPH_REQUIRE(ntm * ntn < (1 << 22), "dph_linear_i8: too many tiles");
-    p.ntn = (int32_t)ntn;
-    p.ntiles = (int32_t)(ntm * ntn);
-    launch_linear<C>(p, a.act == DPH_ACT_GELU, a.residual ? (out32 ? 2 : 1) : 0, out32, stream);
-    return DPH_OK;
+    p.ntn = (int32_t)cdiv(a.N, C::BN);
+    p.ntiles = (int32_t)tiles(C::BM);
+    launch_linear<C>(p, gelu, res, out32, stream);
   };
-  const char* ev = getenv("DPH_I8_TILE");
-  const int sel = ev ? atoi(ev) : 0;
-  if (sel == 0) DPH_TRY(go(mt::Tile<128, 128, 2, 2, 2>{}));
-  if (sel == 1) DPH_TRY(go(mt::Duo<256, 256, 1>{}));
-  if (sel == 2) DPH_TRY(go(mt::Duo<128, 256, 1>{}));
-  if (sel == 3) DPH_TRY(go(mt::Duo<128, 192, 2>{}));
-  if (sel == 4) DPH_TRY(go(mt::Duo<128, 128, 2>{}));
-  if (sel == 5) DPH_TRY(go(mt::Tile<64, 64, 2, 2, 4>{}));
-  if (sel == 6) DPH_TRY(go(mt::Duo<256, 128, 1>{}));
-  if (sel == 7) DPH_TRY(go(mt::Duo<128, 192, 1>{}));
+  if (c64 < c128 && c64 < c256) go(C64{});
+  else if (c128 < c256) go(C128{});
+  else go(C256{});
   return check_launch("dph_linear_i8");
 }

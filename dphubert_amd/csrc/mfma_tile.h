@@ -469,17 +469,20 @@ __device__ __forceinline__ void product_of(const Rows& A, const Rows& B, int32_t
   else product<T, C>(A, B, kbytes, m0, n0, acc, smem, wave, lane, init);
 }
 
-// ---- whole rows in a lane --------------------------------------------------------------------------------------------
-// A wave's 16 x 16 FN strip of acc has 4 columns of each fragment in a lane: 8-byte accesses of 32-byte runs.  Exchanging
-// them between the four groups of 16 lanes (a transpose of groups and fragments, by lane swaps; its own inverse) gives a
-// lane W = 16 (8 where FN = 2) consecutive columns, and a row of the wave 128-byte runs of fp16.
-template <int FN>
+// ---- 16 bytes of a row in a lane -------------------------------------------------------------------------------------
+// A wave's 16 x 16 FN strip of acc has 4 columns of each fragment in a lane: 16-byte accesses of 64-byte runs if they are
+// stored in 32 bits, but 8-byte ones of 32-byte runs in 16.  Exchanging the columns of two fragments between the groups
+// of 16 lanes (by lane swaps; its own inverse) gives a lane 8 consecutive ones, and 64-byte runs of 16-bit numbers.
+// (16 columns a lane, two 16-byte accesses a lane, stored 7984 x 4096 at 2.4 TB/s: what counts is one access's run.)
+template <int FN, int W_>
 struct Strip {
-  static constexpr int W = FN % 4 == 0 ? 16 : 8, NG = 4 * FN / W;   // NG groups of W columns a lane
-  static_assert(FN % 4 == 0 || FN == 2, "whole exchanges");
+  static constexpr int W = W_, NG = 4 * FN / W;   // NG groups of W columns a lane
+  static_assert(W == 4 || (W == 8 && FN % 2 == 0) || (W == 16 && FN % 4 == 0), "whole exchanges");
   // first column of group q in the strip
   static __device__ __forceinline__ int col(int q, int lane) {
-    return W == 16 ? 64 * q + 16 * (lane >> 4) : 16 * ((lane >> 4) & 1) + 8 * (lane >> 5);
+    return W == 4    ? 16 * q + 4 * (lane >> 4)
+           : W == 8  ? 32 * q + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5)
+                     : 64 * q + 16 * (lane >> 4);
   }
   static __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
     const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
@@ -494,20 +497,19 @@ struct Strip {
   // v[4 j + r]: fragment j's column 4 (lane / 16) + r  <->  v[W q + c]: column col(q) + c
   static __device__ __forceinline__ void exchange(uint32_t (&v)[4 * FN]) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (W == 16) {
+    for (int q = 0; q < NG; ++q)
 #pragma unroll
-        for (int q = 0; q < NG; ++q) {
-          uint32_t* a = v + 16 * q + r;
+      for (int r = 0; r < 4; ++r) {
+        uint32_t* a = v + W * q + r;
+        if constexpr (W == 16) {
           swap32(a[0], a[8]);
           swap32(a[4], a[12]);
           swap16(a[0], a[4]);
           swap16(a[8], a[12]);
+        } else if constexpr (W == 8) {
+          swap16(a[0], a[4]);
         }
-      } else {
-        swap16(v[r], v[4 + r]);
       }
-    }
   }
 };
 

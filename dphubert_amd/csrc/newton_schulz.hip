@@ -29,6 +29,9 @@
 #include <type_traits>
 
 
+#ifndef NSW
+#define NSW 16
+#endif
 namespace dph {
 namespace {
 
@@ -272,7 +275,7 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
   const int64_t yoff = (int64_t)z * g.np * g.mp * 2, eoff = (int64_t)z * g.mp * g.mp * 2;
   const int kbytes = (KIND == GRAM ? g.np : g.mp) * 2;
   const int64_t ld = (int64_t)g.mp * 2;
-  using V = mt::Strip<C::FN>;
+  using V = mt::Strip<C::FN, C::FN % 4 == 0 ? NSW : 8>;
   constexpr int NV = 4 * C::FN;
   f32x4_t acc[C::FM][C::FN];
   const int mw = m0 + wave / C::WC * C::WTM + (lane & 15), nw = n0 + wave % C::WC * C::WTN;

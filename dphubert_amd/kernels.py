@@ -8,6 +8,7 @@ inside the library.
 
 import ctypes as C
 import os
+import struct
 from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -503,29 +504,37 @@ def _chk_on(dev, t, name, dtypes, ndim):
 
 def _chk_rows(t, name):
     """[R, K] rows of unit stride that do not overlap; their distance in elements."""
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    R, K = t.shape
+    ld, one = t.stride()
+    if K > 1 and one != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous (strides {t.stride()})")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"{name}: rows overlap (strides {t.stride()})")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    if R > 1:
+        if ld < K:
+            raise ValueError(f"{name}: rows overlap (strides {t.stride()})")
+        return ld
+    return max(ld, K)
+
+
+def _chk_vec(dev, t, name, n):
+    _chk_on(dev, t, name, (F32,), 1)
+    if t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous elements, got shape {tuple(t.shape)}, strides {t.stride()}")
 
 
 def _chk_i8(dev, r, name):
-    """The distance of the rows of an I8Rows in bytes."""
-    _chk_on(dev, r.q, name + ".q", (torch.int8,), 2)
-    _chk_on(dev, r.scale, name + ".scale", (F32,), 1)
-    if r.scale.shape[0] != r.q.shape[0] or not r.scale.is_contiguous():
-        raise ValueError(f"{name}: {r.q.shape[0]} rows and a scale of shape {tuple(r.scale.shape)}, "
-                         f"strides {r.scale.stride()}")
-    R, K = r.q.shape
-    ld = _chk_rows(r.q, name + ".q")
+    """(rows, columns, the distance of the rows in bytes) of an I8Rows."""
+    q, scale = r
+    _chk_on(dev, q, name + ".q", (torch.int8,), 2)
+    R, K = q.shape
+    _chk_vec(dev, scale, name + ".scale", R)
+    ld = _chk_rows(q, name + ".q")
     if R == 1:
-        ld = (ld + 15) // 16 * 16
-    ends = r.q.storage_offset() + (R - 1) * ld + (K + 15) // 16 * 16
-    if R and (ld % 16 or r.q.data_ptr() % 16 or ends > r.q.untyped_storage().nbytes()):
+        ld = _i8_ld(K)
+    if R and (ld % 16 or q.data_ptr() % 16 or
+              q.storage_offset() + (R - 1) * ld + _i8_ld(K) > q.untyped_storage().nbytes()):
         raise ValueError(f"{name}.q: rows must start (and be readable to) a multiple of 16 bytes, as quant_rows_i8 lays "
-                         f"them out; shape {tuple(r.q.shape)}, strides {r.q.stride()}")
-    return ld
+                         f"them out; shape {tuple(q.shape)}, strides {q.stride()}")
+    return R, K, ld
 
 
 def _i8_ld(K: int) -> int:
@@ -553,69 +562,77 @@ def quant_rows_i8(x: torch.Tensor) -> I8Rows:
     return I8Rows(q[:, :K] if ld != K else q, scale)
 
 
+_I8_ARGS = struct.Struct("3qQq2i3QqQqQQqQQQqQq2ifi")      # DphLinearI8Args, filled in one go
+assert _I8_ARGS.size == C.sizeof(_lib.DphLinearI8Args)
+
+
 def _linear_i8(x, w, bias, act, residual, out, out_dtype, ln, keep_norm):
     rows = isinstance(x, I8Rows)
     t = x.q if rows else x
     if not isinstance(t, torch.Tensor):
         raise ValueError("x must be a device tensor (no CPU path)")
-    dev = t.device
-    if rows:
-        ldq = _chk_i8(dev, x, "x")
-    else:
-        _chk_on(dev, x, "x", (BF16, F32), 2)
     if not isinstance(w, I8Rows):
         raise ValueError("w must be an I8Rows (quant_rows_i8 of the nn.Linear weight)")
-    ldw = _chk_i8(dev, w, "w")
-    M, K = t.shape
-    N = w.q.shape[0]
-    if w.q.shape[1] != K:
-        raise ValueError(f"x has rows of {K} elements, w of {w.q.shape[1]}")
+    dev = t.device
+    N, K, ldw = _chk_i8(dev, w, "w")
+    if rows:
+        M, Kx, ldq = _chk_i8(dev, x, "x")
+    else:
+        _chk_on(dev, x, "x", (BF16, F32), 2)
+        M, Kx = x.shape
+        ldx = _chk_rows(x, "x")
+    if Kx != K:
+        raise ValueError(f"x has rows of {Kx} elements, w of {K}")
     if not 1 <= K <= _lib.I8_K_MAX:
         raise ValueError(f"x: rows of 1 to {_lib.I8_K_MAX} elements, got {K}")
     if act not in (ACT_NONE, ACT_GELU):
         raise ValueError(f"act must be ACT_NONE or ACT_GELU, got {act}")
-    a = _lib.DphLinearI8Args()
     if bias is not None:
-        _chk_on(dev, bias, "bias", (F32,), 1)
-        if bias.shape[0] != N or not bias.is_contiguous():
-            raise ValueError(f"bias: expected {N} contiguous elements, got shape {tuple(bias.shape)}")
-        a.bias = ptr(bias)
+        _chk_vec(dev, bias, "bias", N)
+    ldr = 0
     if residual is not None:
         _chk_on(dev, residual, "residual", (BF16, F32), 2)
-        if tuple(residual.shape) != (M, N):
+        if residual.shape[0] != M or residual.shape[1] != N:
             raise ValueError(f"residual: expected {(M, N)}, got {tuple(residual.shape)}")
         out_dtype = residual.dtype
-        a.ldr = _chk_rows(residual, "residual")
-        a.residual, a.residual_f32 = ptr(residual), int(out_dtype == F32)
-    if out_dtype not in (BF16, F32):
+        ldr = _chk_rows(residual, "residual")
+    elif out_dtype not in (BF16, F32):
         raise ValueError(f"out_dtype must be bf16 or fp32, got {out_dtype}")
     norm = None
     with _on_device(dev):
         if out is None:
-            out = torch.empty(M, N, dtype=out_dtype, device=dev)
+            out = torch.empty((M, N), dtype=out_dtype, device=dev)
+            ldo = N
         else:
             _chk_on(dev, out, "out", (out_dtype,), 2)
-            if tuple(out.shape) != (M, N):
+            if out.shape[0] != M or out.shape[1] != N:
                 raise ValueError(f"out: expected {(M, N)}, got {tuple(out.shape)}")
-        a.ldo = _chk_rows(out, "out")
-        a.M, a.N, a.K, a.act = M, N, K, act
-        if not rows:
-            a.x, a.x_f32, a.ldx = ptr(x), int(x.dtype == F32), _chk_rows(x, "x")
-            ldq = _i8_ld(K)
-            ws = torch.empty(M * (ldq + 4), dtype=torch.int8, device=dev)    # q, then the scales
-            a.q, a.q_scale = ws.data_ptr(), ws.data_ptr() + M * ldq
-            if ln is not None:
-                a.ln_weight, a.ln_bias, a.ln_eps = ptr(ln[0]), ptr(ln[1]), ln[2]
-                if keep_norm:
-                    norm = torch.empty(M, K, dtype=BF16, device=dev)
-                    a.norm_out, a.ld_norm = ptr(norm), K
+            ldo = _chk_rows(out, "out")
+        if not M:
+            return out, torch.empty((0, K), dtype=BF16, device=dev) if keep_norm else None
+        if rows:
+            xp, xf, ldx = 0, 0, 0
+            qp, sp = x.q.data_ptr(), x.scale.data_ptr()
         else:
-            a.q, a.q_scale = ptr(x.q), ptr(x.scale)
-        a.ldq = ldq
-        a.w, a.ldw, a.w_scale = ptr(w.q), ldw, ptr(w.scale)
-        a.out, a.out_dtype = ptr(out), OUT_F32 if out_dtype == F32 else OUT_BF16
-        if M:
-            call("dph_linear_i8", C.byref(a), _stream())
+            xp, xf, ldq, qp, sp = x.data_ptr(), x.dtype == F32, _i8_ld(K), 0, 0
+            nbytes = _lib.lib().dph_linear_i8_workspace(M, N, K)
+            if nbytes:
+                ws = torch.empty(nbytes, dtype=torch.int8, device=dev)    # q, then the scales
+                qp = ws.data_ptr()
+                sp = qp + M * ldq
+        lw = lb = np = 0
+        eps = 0.0
+        if ln is not None:
+            lw, lb, eps = ln
+            if keep_norm:
+                norm = torch.empty((M, K), dtype=BF16, device=dev)
+                np = norm.data_ptr()
+        f32 = out_dtype == F32
+        call("dph_linear_i8",
+             _I8_ARGS.pack(M, N, K, xp, ldx, xf, act, lw, lb, np, K, qp, ldq, sp, w.q.data_ptr(), ldw,
+                           w.scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                           0 if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldo, f32,
+                           OUT_F32 if f32 else OUT_BF16, eps, 0), _stream())
     return out, norm
 
 
@@ -644,13 +661,12 @@ def layernorm_linear_i8(x: torch.Tensor, ln_weight: torch.Tensor, ln_bias: torch
     K = x.shape[1]
     if not 1 <= K <= _lib.I8_LN_MAX:
         raise ValueError(f"x: rows of 1 to {_lib.I8_LN_MAX} elements, got {K}")
-    for t, name in ((ln_weight, "ln_weight"), (ln_bias, "ln_bias")):
-        _chk_on(x.device, t, name, (F32,), 1)
-        if t.shape[0] != K or not t.is_contiguous():
-            raise ValueError(f"{name}: expected {K} contiguous elements, got shape {tuple(t.shape)}")
+    _chk_vec(x.device, ln_weight, "ln_weight", K)
+    _chk_vec(x.device, ln_bias, "ln_bias", K)
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    return _linear_i8(x, w, bias, act, None, None, BF16, (ln_weight, ln_bias, float(eps)), keep_norm)
+    return _linear_i8(x, w, bias, act, None, None, BF16, (ln_weight.data_ptr(), ln_bias.data_ptr(), float(eps)),
+                      keep_norm)
 
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)

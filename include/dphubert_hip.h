@@ -679,6 +679,9 @@ typedef struct DphLinearI8Args {
   int32_t reserved;
 } DphLinearI8Args;
 int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream);
+/* bytes that x's integers and scales need (q, rows the next multiple of 16 of K apart, then q_scale); 0: q and q_scale may
+ * be NULL (up to 16 rows are quantised where they are multiplied) */
+int64_t dph_linear_i8_workspace(int64_t M, int64_t N, int64_t K);
 
 /* ---- Newton-Schulz orthogonalisation (ABI 25) ---------------------------------------------------------------------
  * For every matrix G [rows][cols] of the groups (one shape and type each): X0 = G / (|G|_F + eps) (the smaller side

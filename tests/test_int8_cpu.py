@@ -40,9 +40,12 @@ def _args(**kw):
 @pytest.mark.parametrize("kw", [
     dict(M=-1), dict(K=0), dict(N=-2), dict(K=131073, ldq=131088, ldw=131088), dict(M=1 << 40), dict(q=None), dict(ldq=31), dict(ldq=40),
     dict(q=4100), dict(ldq=16), dict(act=7), dict(out_dtype=2), dict(w=None), dict(w=4104), dict(ldw=8), dict(ldw=36), dict(out=None),
-    dict(ldo=3), dict(w_scale=None), dict(q_scale=None), dict(residual=4096, residual_f32=1), dict(x=4096, ldx=31),
+    dict(ldo=3), dict(residual=4096, ldr=3), dict(w_scale=None), dict(q_scale=None), dict(residual=4096, residual_f32=1), dict(x=4096, ldx=31),
     dict(x=4096, ldx=32, ln_weight=4096), dict(x=4096, ldx=4096, ln_weight=4096, ln_bias=4096, K=2049, ldq=2064, ldw=2064),
-    dict(x=4096, ldx=32, ln_weight=4096, ln_bias=4096, ldq=1024),
+    dict(M=17, x=4096, ldx=32, ln_weight=4096, ln_bias=4096, ldq=1024), dict(M=17, x=4096, ldx=32, q=None),
+    dict(x=4096, ldx=32, ln_weight=4096, ln_bias=4096, norm_out=4096, ld_norm=31), dict(x=4096, ldx=32, w=None),
+    dict(x=4096, ldx=32, ln_weight=4096, ln_bias=4096, out_dtype=K.OUT_F32),
+    dict(x=4096, ldx=32, ln_weight=4096, ln_bias=4096, residual=4096, ldr=4),
 ])
 def test_c_entry_refuses(kw):
     """The C entry's own checks (nothing is launched: there is no device here)."""
@@ -56,6 +59,13 @@ def test_c_quant_refuses(kw):
     d = dict(x=4096, f32=0, rows=4, K=32, ldx=32, q=4096, ldq=32, scale=4096)
     d.update(kw)
     assert _lib.lib().dph_quant_rows_i8(d["x"], d["f32"], d["rows"], d["K"], d["ldx"], d["q"], d["ldq"], d["scale"], None) == -1
+
+
+def test_workspace():
+    """Nothing for up to 16 rows that fit the LDS, else the integers (rows of whole 16 bytes) and the scales."""
+    ws = _lib.lib().dph_linear_i8_workspace
+    assert ws(1, 8, 1024) == ws(16, 1, 64) == ws(0, 8, 8) == ws(16, 5, 3500) == 0
+    assert ws(17, 8, 33) == 17 * (48 + 4) and ws(16, 8, 4096) == 16 * (4096 + 4)
 
 
 def test_c_empty_calls():
