@@ -80,6 +80,11 @@ class DphNsGroup(C.Structure):
     _fields_ = [("rows", i64), ("cols", i64), ("count", i64), ("out", vp), ("f32", i32), ("reserved", i32)]
 
 
+class DphMuonSlot(C.Structure):
+    _fields_ = [("param", vp), ("grad", vp), ("momentum", vp), ("update", vp), ("dir", vp), ("img", vp), ("n", i64),
+                ("scale", f32), ("group", i32)]
+
+
 I8_K_MAX = 131072
 I8_LN_MAX = 2048
 
@@ -192,6 +197,8 @@ _SIGS = {
     "dph_newton_schulz_workspace": ([C.POINTER(DphNsGroup), i64], i64),
     "dph_newton_schulz": ([C.POINTER(DphNsMat), C.POINTER(DphNsGroup), i64, i64, C.POINTER(f32), f32, vp, i64, S],
                           C.c_int),
+    "dph_muon_momentum": ([vp, i64, vp, vp, i64, vp, vp, i64, C.c_int, vp, f32, S], C.c_int),
+    "dph_muon_apply": ([vp, i64, vp, vp, i64, vp, vp, i64, S], C.c_int),
     "dph_set_rng_epoch": ([vp], C.c_int),
     "dph_event_create": ([C.POINTER(vp)], C.c_int),
     "dph_event_record": ([vp, S], C.c_int),
@@ -211,7 +218,7 @@ _lib = None
 #     DphGemmArgs.sk_* + dph_gemm_sk_plan: the persistent stream-K 256 x 256 GEMM;
 # 24: dph_attention_bwd_qv / dph_attention_bwd_relpos_qv + dph_attention_bwd_qv_workspace: the q / v bias
 #     gradients summed inside the attention backward;
-# 25: dph_quant_rows_i8 / dph_linear_i8: 8-bit integer products; dph_newton_schulz)
+# 25: dph_quant_rows_i8 / dph_linear_i8: 8-bit integer products; dph_newton_schulz, dph_muon_momentum / _apply)
 ABI_VERSION = 25
 
 

@@ -68,6 +68,12 @@ def _common_args(p: argparse.ArgumentParser, lr: float, warmup: int, max_updates
                         "(--synthetic_utterances) batches, off for bucketed corpus batches (their length varies)")
     p.add_argument("--grad_comm_dtype", default="fp32", choices=["fp32", "bf16"],
                    help="payload of the data-parallel gradient all-reduce (bf16 halves the xGMI bytes)")
+    p.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"],
+                   help="muon: the student encoder's projection matrices move along the orthogonal factor of their "
+                        "momentum (Newton-Schulz), everything else by AdamW; the learning rate carries over")
+    p.add_argument("--muon_momentum", default=0.95, type=float)
+    p.add_argument("--teacher_int8", action="store_true",
+                   help="run the frozen teacher's encoder products in 8-bit integers (one scale a token and a channel)")
     p.add_argument("--reshuffle_each_epoch", action="store_true",
                    help="new batch order every epoch (the reference's DistributedBatchSampler permutes once, so by "
                         "default every epoch repeats epoch 0's order, as the reference does)")
@@ -235,6 +241,8 @@ def _train(args, module, world, rank, dev):
     from . import ops
     ops.manual_seed(2022 + rank)
     module = module.to(dev)
+    if args.teacher_int8:
+        module.teacher_model.quantize_int8()
     graphs = args.graphs == "on" or (args.graphs == "auto" and args.synthetic_utterances > 0)
     trainer = Trainer(module, clip_norm=args.clip_norm, accum_grad=args.accum_grad, graphs=graphs,
                       grad_dtype=torch.bfloat16 if args.grad_comm_dtype == "bf16" else torch.float32)
@@ -349,7 +357,7 @@ def distill_main(argv=None):
                            reg_learning_rate=args.reg_learning_rate, target_sparsity=args.target_sparsity,
                            sparsity_warmup_updates=args.sparsity_warmup_updates, tsv_dir=args.tsv_dir or ".",
                            train_subset=args.train_subset, seconds_per_batch=args.seconds_per_batch,
-                           num_workers=args.num_workers)
+                           num_workers=args.num_workers, optimizer=args.optimizer, muon_momentum=args.muon_momentum)
     _train(args, module, world, rank, dev)
 
 
@@ -383,7 +391,8 @@ def final_distill_main(argv=None):
                            distill_loss=DistillLoss(args.l2_weight, args.l1_weight, args.cos_weight, args.cos_type),
                            learning_rate=args.learning_rate, weight_decay=args.weight_decay,
                            warmup_updates=args.warmup_updates, max_updates=args.max_updates, use_reg=False,
-                           reg_learning_rate=None, target_sparsity=None, sparsity_warmup_updates=None)
+                           reg_learning_rate=None, target_sparsity=None, sparsity_warmup_updates=None,
+                           optimizer=args.optimizer, muon_momentum=args.muon_momentum)
     _train(args, module, world, rank, dev)
 
 

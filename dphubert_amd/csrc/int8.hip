@@ -643,14 +643,9 @@ extern "C" int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream) {
     else launch_small<bf16_t>(sm, gelu, res, out32, stream);
     return check_launch("dph_linear_i8");
   }
-  // Tiles of 256 x 256 (one a CU), 128 x 128 or 64 x 64 (two): whichever needs least time by the rounds that its tiles take
-  // on 256 CUs, a round of theirs counting 1, 0.55 and 0.27.  Measured, the product alone: 7984 x 1024 x 4096 62 / 45 / 66
-  // us, 8192 x 8192 x 8192 398 / 518 us / -, 7984 x 2304 x 768 32 / 24 / 36 us, 1497 x 768 x 1533 37 / 16 / 15 us.
-  using C256 = mt::Duo<256, 256, 1>;
-  using C128 = mt::Duo<128, 128, 2>;
-  using C64 = mt::Tile<64, 64, 2, 2, 4>;
+  // Measured on tiles of 256 / 128 / 64, the product alone: 7984 x 1024 x 4096 62 / 45 / 66 us, 8192 x 8192 x 8192 398 / 518 us
+  // / -, 7984 x 2304 x 768 32 / 24 / 36 us, 1497 x 768 x 1533 37 / 16 / 15 us
   auto tiles = [&](int b) { return cdiv(a.M, b) * cdiv(a.N, b); };
-  const double c256 = (double)cdiv(tiles(256), 256), c128 = 0.55 * cdiv(tiles(128), 512), c64 = 0.27 * cdiv(tiles(64), 512);
   DPH_REQUIRE(tiles(256) < (1 << 22), "dph_linear_i8: too many tiles");
   auto go = [&](auto c) {
     using C = decltype(c);
@@ -658,8 +653,9 @@ extern "C" int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream) {
     p.ntiles = (int32_t)tiles(C::BM);
     launch_linear<C>(p, gelu, res, out32, stream);
   };
-  if (c64 < c128 && c64 < c256) go(C64{});
-  else if (c128 < c256) go(C128{});
-  else go(C256{});
+  const int tile = mt::choose_tile(tiles(256), tiles(128), tiles(64));
+  if (tile == 64) go(mt::C64{});
+  else if (tile == 128) go(mt::C128{});
+  else go(mt::C256{});
   return check_launch("dph_linear_i8");
 }

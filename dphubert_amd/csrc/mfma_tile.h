@@ -514,10 +514,26 @@ struct Strip {
 };
 
 // Workgroups go to the 8 XCDs in turn: block b of n works on a contiguous range of tiles per XCD, so the tiles of one
-// L2 share their operands' rows
-__device__ __forceinline__ int xcd_tile(int b, int n) {
-  const int q = n >> 3, r = n & 7, x = b & 7, i = b >> 3;
-  return x * q + min(x, r) + i;
+// L2 share their operands' rows (reverse: each XCD its own range backwards)
+__device__ __forceinline__ int xcd_tile(int b, int n, bool reverse = false) {
+  const int q = n >> 3, r = n & 7, x = b & 7, i = b >> 3, size = q + (x < r ? 1 : 0);
+  return x * q + min(x, r) + (reverse ? size - 1 - i : i);
+}
+
+// Which tiles a product of so many of each takes: 256 x 256 (one workgroup a CU), 128 x 128 or 64 x 64 (two).  A CU's work
+// is counted in rounds of 256 CUs: a 256 x 256 tile 1, two tiles of 128 x 128 side by side 0.58 and one alone 0.36, of 64 x
+// 64 0.33 and 0.22 (measured on K of 512 to 4096: the larger the tile, the fewer bytes pass the LDS a product, but the
+// more of the chip idles in the last round).  A negative count: not available.
+struct C256 : Duo<256, 256, 1> {};
+struct C128 : Duo<128, 128, 2> {};
+struct C64 : Tile<64, 64, 2, 2, 4> {};
+inline double pairs(int64_t tiles, double two, double one) {
+  const int64_t n = cdiv(tiles, 256);
+  return tiles < 0 ? 1e30 : (double)(n / 2) * two + (double)(n % 2) * one;
+}
+inline int choose_tile(int64_t t256, int64_t t128, int64_t t64) {
+  const double c256 = (double)cdiv(t256, 256), c128 = pairs(t128, 0.58, 0.36), c64 = pairs(t64, 0.33, 0.22);
+  return c64 < c128 && c64 < c256 ? 64 : c128 < c256 ? 128 : 256;
 }
 
 }  // namespace mt

@@ -15,7 +15,7 @@
 //     leaves in e4m3), so weak directions are not lost in the rounding of strong ones.  The products read the fp16 alone.
 //   * In the last two steps the singular values are near 1 and a X + b A X + c A^2 X cancel by a factor of 5.  There the
 //     polynomial is expanded about d = 1:  E = A - d I,  F = (b + 2 c d) E + c E^2,  X <- (a + b d + c d^2) X + F X,
-//     the same products on numbers near 0, whose roundings are small.
+//     the same products on numbers near 0, whose roundings are small (the last coefficient is put into F's diagonal).
 // In large matrices an operand's roundings average out; up to NS_SPLIT rows they need not (a 1 x 1 matrix is off by
 // 8e-3), and there every operand is two fp16 and every product three: h h + l h + h l.  Such matrices are a few tiles:
 // launches, not products, set their time.
@@ -100,7 +100,8 @@ struct Mats {
   Mat m[NS_MATS];
 };
 struct Step {
-  float d, fe, fq, mu;     // E = A - d I;  F = fe E + fq E^2;  Y <- mu Y + Y F
+  float d, fe, fq, mu, fd; // E = A - d I;  F = fe E + fq E^2 + fd I;  Y <- mu Y + Y F
+  int32_t reverse;         // tiles from the last to the first
   int32_t cur;             // which y is read
   int32_t lo_in, lo_out;   // Y's 8 bits more are read, written
 };
@@ -247,7 +248,9 @@ template <int KIND, bool SPLIT, class C>
 __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups gs, const Step st) {
   __shared__ __align__(16) char smem[C::LDS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  int t = mt::xcd_tile((int)blockIdx.x, (int)gridDim.x);
+  // every other launch goes through the matrices backwards: it starts with what the last one wrote last, which the
+  // caches still hold (each XCD keeps its own matrices: its L2 has them)
+  int t = mt::xcd_tile((int)blockIdx.x, (int)gridDim.x, st.reverse != 0);
   int k = 0;
   while (k + 1 < gs.ng && gs.first[k + 1] <= t) ++k;
   const Group& g = gs.g[k];
@@ -282,7 +285,7 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
   const int M = SYM ? g.mp : g.np, N = g.mp;      // (what lies past m and n is zero, and stays zero)
   // the sums start from 0, or from mu Y, whose rows are about to be read as an operand anyway
   auto init = [&]() {
-    if constexpr (SYM) {
+    if (SYM || st.mu == 0.f) {
       mt::clear<T, C>(acc);
     } else {
       const float mu = st.mu * NS_E;
@@ -381,7 +384,7 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
               }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[c + r] += st.fe * e[r];
+            for (int r = 0; r < 4; ++r) v[c + r] += st.fe * e[r] + (m == n0q + c + r && m < g.m ? NS_E * st.fd : 0.f);
           }
         }
 #pragma unroll
@@ -536,22 +539,18 @@ int launch_tiles(const Groups& all, const Step& st, hipStream_t stream) {
   return check_launch("dph_newton_schulz");
 }
 
-// Tiles of 256 x 256 (one a CU), 128 x 128 or 64 x 64 (two): whichever needs least time by the rounds that its tiles take
-// on 256 CUs, a round of theirs counting 1, 0.58 and 0.27.  Measured, a whole call: 24 of 1024 x 4096 2.63 / 2.88 / 4.61
-// ms, 48 of 768 x 768 1.11 / 0.88 / 1.20 ms, one of 768 x 768 472 / 221 / 147 us, 8 of 448 x 768 396 / 188 / 152 us.
+// Measured, a whole call with all products on tiles of 256 / 128 / 64: 24 of 1024 x 4096 2.63 / 2.88 / 4.61 ms, 48 of 768 x
+// 768 1.11 / 0.88 / 1.20 ms, one of 768 x 768 472 / 221 / 147 us, 8 of 448 x 768 396 / 188 / 152 us.
 template <int KIND>
 int launch_product(const Groups& gs, const Step& st, hipStream_t stream) {
-  using C256 = mt::Duo<256, 256, 1>;
-  using C128 = mt::Duo<128, 128, 2>;
-  using C64 = mt::Tile<64, 64, 2, 2, 4>;
-  DPH_TRY((launch_tiles<KIND, true, C64>(gs, st, stream)));
+  DPH_TRY((launch_tiles<KIND, true, mt::C64>(gs, st, stream)));
   Groups some = {};
-  const int64_t t256 = choose<KIND, false, C256>(gs, &some), t128 = choose<KIND, false, C128>(gs, &some),
-                t64 = choose<KIND, false, C64>(gs, &some);
-  const double c256 = (double)cdiv(t256, 256), c128 = 0.58 * cdiv(t128, 512), c64 = 0.27 * cdiv(t64, 512);
-  if (t64 >= 0 && c64 < c128 && c64 < c256) return launch_tiles<KIND, false, C64>(gs, st, stream);
-  if (t128 >= 0 && c128 < c256) return launch_tiles<KIND, false, C128>(gs, st, stream);
-  return launch_tiles<KIND, false, C256>(gs, st, stream);
+  const int64_t t256 = choose<KIND, false, mt::C256>(gs, &some), t128 = choose<KIND, false, mt::C128>(gs, &some),
+                t64 = choose<KIND, false, mt::C64>(gs, &some);
+  const int tile = t256 < 0 ? 256 : mt::choose_tile(t256, t128, t64);
+  if (tile == 64) return launch_tiles<KIND, false, mt::C64>(gs, st, stream);
+  if (tile == 128) return launch_tiles<KIND, false, mt::C128>(gs, st, stream);
+  return launch_tiles<KIND, false, mt::C256>(gs, st, stream);
 }
 
 // up to NS_GROUPS groups, whose matrices start at mats
@@ -605,14 +604,21 @@ int run_groups(const DphNsMat* mats, const DphNsGroup* groups, int ng, int steps
     st.d = late ? 1.f : 0.f;
     st.fe = c[1] + 2.f * c[2] * st.d;
     st.fq = c[2];
-    st.mu = c[0] + c[1] * st.d + c[2] * st.d * st.d;
+    // near the end mu is below 1 and goes into F's diagonal, whose rounding it does not make worse, and Y is read as an
+    // operand only; before, mu Y is added in as many bits as Y has
+    const float mu = c[0] + c[1] * st.d + c[2] * st.d * st.d;
+    st.mu = late ? 0.f : mu;
+    st.fd = late ? mu : 0.f;
     st.cur = i & 1;
     st.lo_in = !late;
     st.lo_out = !(steps - i - 1 <= 2 && steps >= 4);
     DPH_TRY(launch_product<GRAM>(gs, st, stream));
+    st.reverse ^= 1;
     DPH_TRY(launch_product<POLY>(gs, st, stream));
+    st.reverse ^= 1;
     if (i + 1 < steps) DPH_TRY(launch_product<UPDATE>(gs, st, stream));
     else DPH_TRY(launch_product<LAST>(gs, st, stream));
+    st.reverse ^= 1;
   }
   return DPH_OK;
 }

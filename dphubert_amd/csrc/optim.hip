@@ -141,6 +141,97 @@ __global__ void __launch_bounds__(256) adamw_kernel(const DphTensorSlot* __restr
   }
 }
 
+// Muon: momentum and the matrix that is orthogonalised, then the step along its orthogonal factor.  Both passes are bound
+// by memory: 20 and 12 bytes a parameter (and 2 of the image).
+__global__ void __launch_bounds__(256) muon_momentum_kernel(const DphMuonSlot* __restrict__ slots,
+                                                            const int64_t* __restrict__ cslot,
+                                                            const int64_t* __restrict__ cstart, Groups G,
+                                                            const DphAdamDyn* __restrict__ dyn, int nesterov,
+                                                            const float* __restrict__ sumsq, float max_norm) {
+  const DphMuonSlot sl = slots[cslot[blockIdx.x]];
+  if (!sl.grad) return;
+  const DphAdamGroup gr = dyn ? dyn->g[sl.group] : G.g[sl.group];
+  float clip = 1.0f;
+  if (sumsq && max_norm > 0.f) clip = fminf(max_norm / (sqrtf(*sumsq) + 1e-6f), 1.0f);
+  const float b = gr.beta1, bc = 1.0f - gr.beta1;
+  auto upd = [&](float& g, float& m) {
+    g *= clip;
+    m = m + (g - m) * bc;
+    return nesterov ? g + (m - g) * b : m;
+  };
+  const int64_t s0 = cstart[blockIdx.x], s1 = min(sl.n, s0 + CHUNK);
+  int64_t i0 = s0;
+  const uintptr_t al = reinterpret_cast<uintptr_t>(sl.grad + s0) | reinterpret_cast<uintptr_t>(sl.momentum + s0) |
+                       reinterpret_cast<uintptr_t>(sl.update + s0);
+  if ((al & 15) == 0) {
+    const int64_t n4 = (s1 - s0) >> 2;
+    float4* g4 = reinterpret_cast<float4*>(sl.grad + s0);
+    float4* m4 = reinterpret_cast<float4*>(sl.momentum + s0);
+    float4* u4 = reinterpret_cast<float4*>(sl.update + s0);
+    for (int64_t j = threadIdx.x; j < n4; j += 256) {
+      float4 g = g4[j], m = m4[j], u;
+      u.x = upd(g.x, m.x);
+      u.y = upd(g.y, m.y);
+      u.z = upd(g.z, m.z);
+      u.w = upd(g.w, m.w);
+      m4[j] = m;
+      u4[j] = u;
+      if (clip < 1.0f) g4[j] = g;
+    }
+    i0 = s0 + 4 * n4;
+  }
+  for (int64_t i = i0 + threadIdx.x; i < s1; i += 256) {
+    float g = sl.grad[i], m = sl.momentum[i];
+    sl.update[i] = upd(g, m);
+    sl.momentum[i] = m;
+    if (clip < 1.0f) sl.grad[i] = g;
+  }
+}
+
+__global__ void __launch_bounds__(256) muon_apply_kernel(const DphMuonSlot* __restrict__ slots,
+                                                         const int64_t* __restrict__ cslot,
+                                                         const int64_t* __restrict__ cstart, Groups G,
+                                                         const DphAdamDyn* __restrict__ dyn) {
+  const DphMuonSlot sl = slots[cslot[blockIdx.x]];
+  if (!sl.grad) return;
+  const DphAdamGroup gr = dyn ? dyn->g[sl.group] : G.g[sl.group];
+  const float keep = 1.0f - gr.lr * gr.weight_decay, step = gr.lr * sl.scale;
+  const int64_t s0 = cstart[blockIdx.x], s1 = min(sl.n, s0 + CHUNK);
+  int64_t i0 = s0;
+  const uintptr_t al = reinterpret_cast<uintptr_t>(sl.param + s0) | 2 * reinterpret_cast<uintptr_t>(sl.dir + s0) |
+                       (sl.img ? 2 * reinterpret_cast<uintptr_t>(sl.img + s0) : 0);
+  if ((al & 15) == 0) {
+    const int64_t n4 = (s1 - s0) >> 2;
+    float4* p4 = reinterpret_cast<float4*>(sl.param + s0);
+    for (int64_t j = threadIdx.x; j < n4; j += 256) {
+      float4 p = p4[j];
+      const uint2 d = *reinterpret_cast<const uint2*>(sl.dir + s0 + 4 * j);
+      p.x = p.x * keep - step * __uint_as_float(d.x << 16);
+      p.y = p.y * keep - step * __uint_as_float(d.x & 0xffff0000u);
+      p.z = p.z * keep - step * __uint_as_float(d.y << 16);
+      p.w = p.w * keep - step * __uint_as_float(d.y & 0xffff0000u);
+      p4[j] = p;
+      if (sl.img) *reinterpret_cast<uint2*>(sl.img + s0 + 4 * j) = make_uint2(pack2bf(p.x, p.y), pack2bf(p.z, p.w));
+    }
+    i0 = s0 + 4 * n4;
+  }
+  for (int64_t i = i0 + threadIdx.x; i < s1; i += 256) {
+    const float p = sl.param[i] * keep - step * bf2f(sl.dir[i]);
+    sl.param[i] = p;
+    if (sl.img) sl.img[i] = f2bf(p);
+  }
+}
+
+int muon_groups(const char* who, const DphMuonSlot* slots, int64_t n_slots, const int64_t* cslot, const int64_t* cstart,
+                int64_t n_chunks, const DphAdamDyn* dyn, const DphAdamGroup* groups, int64_t n_groups, Groups* G) {
+  DPH_REQUIRE(slots && cslot && cstart && n_slots > 0 && n_chunks > 0 && n_chunks < ((int64_t)1 << 24), "%s: bad args", who);
+  DPH_REQUIRE(dyn || (groups && n_groups >= 1 && n_groups <= MAX_GROUPS), "%s: need dyn or groups", who);
+  *G = Groups{};
+  if (!dyn)
+    for (int i = 0; i < MAX_GROUPS; ++i) G->g[i] = groups[i < n_groups ? i : 0];
+  return DPH_OK;
+}
+
 }  // namespace
 }  // namespace dph
 
@@ -192,4 +283,25 @@ extern "C" int dph_adamw_step_img(const DphTensorSlot* slots, int64_t n_slots, c
   hipLaunchKernelGGL(adamw_kernel, dim3((unsigned)n_chunks), dim3(256), 0, stream, slots, chunk_slot, chunk_start, G,
                      dyn ? 1.0f : (float)step, dyn, sumsq, max_norm, img);
   return check_launch("dph_adamw_step_img");
+}
+
+extern "C" int dph_muon_momentum(const DphMuonSlot* slots, int64_t n_slots, const int64_t* chunk_slot,
+                                 const int64_t* chunk_start, int64_t n_chunks, const DphAdamDyn* dyn,
+                                 const DphAdamGroup* groups, int64_t n_groups, int nesterov, const float* sumsq,
+                                 float max_norm, hipStream_t stream) {
+  Groups G;
+  DPH_TRY(muon_groups("dph_muon_momentum", slots, n_slots, chunk_slot, chunk_start, n_chunks, dyn, groups, n_groups, &G));
+  hipLaunchKernelGGL(muon_momentum_kernel, dim3((unsigned)n_chunks), dim3(256), 0, stream, slots, chunk_slot,
+                     chunk_start, G, dyn, nesterov, sumsq, max_norm);
+  return check_launch("dph_muon_momentum");
+}
+
+extern "C" int dph_muon_apply(const DphMuonSlot* slots, int64_t n_slots, const int64_t* chunk_slot,
+                              const int64_t* chunk_start, int64_t n_chunks, const DphAdamDyn* dyn,
+                              const DphAdamGroup* groups, int64_t n_groups, hipStream_t stream) {
+  Groups G;
+  DPH_TRY(muon_groups("dph_muon_apply", slots, n_slots, chunk_slot, chunk_start, n_chunks, dyn, groups, n_groups, &G));
+  hipLaunchKernelGGL(muon_apply_kernel, dim3((unsigned)n_chunks), dim3(256), 0, stream, slots, chunk_slot, chunk_start,
+                     G, dyn);
+  return check_launch("dph_muon_apply");
 }

@@ -672,55 +672,73 @@ def layernorm_linear_i8(x: torch.Tensor, ln_weight: torch.Tensor, ln_bias: torch
 NS_COEFFS = (3.4445, -4.7750, 2.0315)
 
 
+class NewtonSchulzPlan:
+    """The orthogonalisation of one list of matrices, run as often as their contents change (an optimiser's updates): the
+    arguments are checked once, results (``out``, bf16, the matrices' shapes) and workspace are kept.  Runs of one plan
+    are ordered by whoever makes them (one stream, or events): they share both."""
+
+    def __init__(self, mats: Sequence[torch.Tensor], *, steps: int = 5, coeffs: Sequence[float] = NS_COEFFS,
+                 eps: float = 1e-7):
+        mats = list(mats)
+        if not mats:
+            raise ValueError("mats is empty")
+        dev = mats[0].device if isinstance(mats[0], torch.Tensor) else None
+        if not 1 <= int(steps) <= 64:
+            raise ValueError(f"steps must be 1 to 64, got {steps}")
+        if len(coeffs) != 3:
+            raise ValueError(f"coeffs are (a, b, c), got {coeffs}")
+        if not eps >= 0.0:
+            raise ValueError(f"eps must not be negative, got {eps}")
+        places = {}
+        for i, t in enumerate(mats):
+            _chk_on(dev, t, f"mats[{i}]", (BF16, F32), 2)
+            R, K = t.shape
+            if not (R and K):
+                raise ValueError(f"mats[{i}] is empty: {tuple(t.shape)}")
+            s0, s1 = t.stride()
+            by_row = (s1 == 1 or K == 1) and (s0 >= K or R == 1)
+            if not by_row and not ((s0 == 1 or R == 1) and (s1 >= R or K == 1)):
+                raise ValueError(f"mats[{i}]: rows or columns must be contiguous and apart, strides {t.stride()}")
+            # (the stride of a dimension of one element is whatever the view says: it is never used)
+            places.setdefault((R, K, t.dtype), []).append(
+                (i, t.data_ptr()) + ((max(s0, K), 1) if by_row else (1, max(s1, R))))
+        self.device, self.mats = dev, mats
+        self._arr = (_lib.DphNsMat * len(mats))()
+        self._grp = (_lib.DphNsGroup * len(places))()
+        self._steps, self._eps, self._coeffs = int(steps), float(eps), (C.c_float * 3)(*coeffs)
+        self.out = [None] * len(mats)
+        with _on_device(dev):
+            k = 0
+            for g, ((R, K, dt), at) in zip(self._grp, places.items()):
+                res = torch.empty(len(at), R, K, dtype=BF16, device=dev)
+                g.rows, g.cols, g.count, g.out, g.f32 = R, K, len(at), res.data_ptr(), int(dt == F32)
+                for (i, p, rs, cs), o in zip(at, res.unbind()):
+                    self.out[i] = o
+                    self._arr[k] = (p, rs, cs)
+                    k += 1
+            nbytes = _lib.lib().dph_newton_schulz_workspace(self._grp, len(self._grp))
+            if nbytes < 0:
+                _lib.check(-1, "dph_newton_schulz_workspace")
+            self._ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+
+    def run(self) -> List[torch.Tensor]:
+        with _on_device(self.device):
+            call("dph_newton_schulz", self._arr, self._grp, len(self._grp), self._steps, self._coeffs, self._eps,
+                 ptr(self._ws), self._ws.numel(), _stream())
+        return self.out
+
+
 def newton_schulz(mats: Sequence[torch.Tensor], *, steps: int = 5, coeffs: Sequence[float] = NS_COEFFS,
                   eps: float = 1e-7) -> List[torch.Tensor]:
     """The orthogonal factor of every matrix of the list, approximately: ``steps`` quintic Newton-Schulz steps
     X <- a X + (b A + c A^2) X, A = X X^T, from X = G / (|G|_F + eps) (of G^T where G is taller than wide).
 
     mats: 2-D tensors of one device, bf16 or fp32, of any shapes and row strides (a transposed view will do).  Returns
-    bf16 tensors of the same shapes.  Matrices of one shape share launches, so hand in a whole model's at once.  The
+    bf16 tensors of the same shapes.  Matrices of all shapes share launches, so hand in a whole model's at once.  The
     results are within about two bf16 roundings of the iteration in 64 bits (newton_schulz.hip)."""
     mats = list(mats)
     if not mats:
+        if not 1 <= int(steps) <= 64:
+            raise ValueError(f"steps must be 1 to 64, got {steps}")
         return []
-    dev = mats[0].device if isinstance(mats[0], torch.Tensor) else None
-    if not 1 <= int(steps) <= 64:
-        raise ValueError(f"steps must be 1 to 64, got {steps}")
-    if len(coeffs) != 3:
-        raise ValueError(f"coeffs are (a, b, c), got {coeffs}")
-    if not eps >= 0.0:
-        raise ValueError(f"eps must not be negative, got {eps}")
-    places = {}
-    for i, t in enumerate(mats):
-        _chk_on(dev, t, f"mats[{i}]", (BF16, F32), 2)
-        R, K = t.shape
-        if not (R and K):
-            raise ValueError(f"mats[{i}] is empty: {tuple(t.shape)}")
-        s0, s1 = t.stride()
-        if not ((s1 == 1 or K == 1) and (s0 >= K or R == 1)) and not ((s0 == 1 or R == 1) and (s1 >= R or K == 1)):
-            raise ValueError(f"mats[{i}]: rows or columns must be contiguous and apart, strides {t.stride()}")
-        places.setdefault((R, K, t.dtype), []).append(i)
-    arr = (_lib.DphNsMat * len(mats))()
-    grp = (_lib.DphNsGroup * len(places))()
-    out = [None] * len(mats)
-    with _on_device(dev):
-        k = 0
-        for gi, ((R, K, dt), at) in enumerate(places.items()):
-            res = torch.empty(len(at), R, K, dtype=BF16, device=dev)
-            grp[gi].rows, grp[gi].cols, grp[gi].count = R, K, len(at)
-            grp[gi].out, grp[gi].f32 = res.data_ptr(), int(dt == F32)
-            for i, o in zip(at, res.unbind()):
-                out[i] = o
-                s0, s1 = mats[i].stride()
-                by_row = (s1 == 1 or K == 1) and (s0 >= K or R == 1)
-                arr[k].p = mats[i].data_ptr()
-                # (the stride of a dimension of one element is whatever the view says: it is never used)
-                arr[k].row_stride, arr[k].col_stride = (max(s0, K), 1) if by_row else (1, max(s1, R))
-                k += 1
-        nbytes = _lib.lib().dph_newton_schulz_workspace(grp, len(places))
-        if nbytes < 0:
-            _lib.check(-1, "dph_newton_schulz_workspace")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        call("dph_newton_schulz", arr, grp, len(places), int(steps), (C.c_float * 3)(*coeffs), float(eps), ptr(ws),
-             nbytes, _stream())
-    return out
+    return NewtonSchulzPlan(mats, steps=steps, coeffs=coeffs, eps=eps).run()

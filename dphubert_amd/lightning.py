@@ -23,7 +23,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-from .optim import FusedAdamW, LinearDecayLRScheduler
+from .optim import FusedAdamW, FusedMuon, LinearDecayLRScheduler
 from .wav2vec2.model import Wav2Vec2Model
 
 __all__ = ["DistillLoss", "DistillModule", "LinearDecayLRScheduler"]
@@ -97,8 +97,13 @@ class DistillModule(nn.Module):
                  learning_rate: float, weight_decay: float, warmup_updates: int, max_updates: int, use_reg: bool,
                  reg_learning_rate: Optional[float], target_sparsity: Optional[float],
                  sparsity_warmup_updates: Optional[int], tsv_dir: Union[str, pathlib.Path] = ".",
-                 train_subset: str = "train100", seconds_per_batch: float = 160.0, num_workers: int = 0):
+                 train_subset: str = "train100", seconds_per_batch: float = 160.0, num_workers: int = 0,
+                 optimizer: str = "adamw", muon_momentum: float = 0.95):
         super().__init__()
+        if optimizer not in ("adamw", "muon"):
+            raise ValueError(f"optimizer must be adamw or muon, got {optimizer}")
+        self.optimizer_name = optimizer
+        self.muon_momentum = muon_momentum
         self.teacher_model = teacher_model
         self.student_model = student_model
         self.original_num_params = sum(p.numel() for p in teacher_model.parameters())
@@ -153,6 +158,8 @@ class DistillModule(nn.Module):
         # nodes, bound to the stream they were created on) alive into the next step / a graph capture
         self.logged.update({k: v.detach() if torch.is_tensor(v) else v for k, v in d.items()})
 
+    MUON_LINEARS = ("q_proj", "k_proj", "v_proj", "out_proj", "intermediate_dense", "output_dense")
+
     def configure_optimizers(self, clip_norm: Optional[float] = None):
         main_params = [p for n, p in self.student_model.named_parameters() if "log_alpha" not in n and p.requires_grad]
         main_params.extend(list(self.distill_linear_projs.parameters()))
@@ -161,6 +168,14 @@ class DistillModule(nn.Module):
             if id(p) not in seen:
                 seen.add(id(p))
                 mp.append(p)
+        # optimizer="muon": the student encoder layers' projection matrices (attention and feed-forward) take the Muon step
+        # with the main group's learning rate and decay, in a group of their own behind the others
+        mats = []
+        if self.optimizer_name == "muon":
+            mats = [p for lay in self.student_model.encoder.transformer.layers for n, p in lay.named_parameters()
+                    if p.requires_grad and p.dim() == 2 and n.rsplit(".", 2)[-2] in self.MUON_LINEARS]
+            ids = {id(p) for p in mats}
+            mp = [p for p in mp if id(p) not in ids]
         pgs = [{"params": mp, "lr": self.learning_rate, "weight_decay": self.weight_decay, "name": "main_params"}]
         if self.use_reg:
             pgs.extend([
@@ -169,7 +184,12 @@ class DistillModule(nn.Module):
                 {"params": [self.lambda1, self.lambda2], "lr": -self.reg_learning_rate, "weight_decay": 0.0,
                  "name": "lambda"},
             ])
-        optimizer = FusedAdamW(pgs, max_grad_norm=clip_norm)
+        if mats:
+            pgs.append({"params": mats, "lr": self.learning_rate, "weight_decay": self.weight_decay, "name": "muon",
+                        "muon": True, "momentum": self.muon_momentum})
+            optimizer = FusedMuon(pgs, max_grad_norm=clip_norm)
+        else:
+            optimizer = FusedAdamW(pgs, max_grad_norm=clip_norm)
         lr_scheduler = LinearDecayLRScheduler(optimizer, warmup_updates=self.warmup_updates,
                                               max_updates=self.max_updates)
         return {"optimizer": optimizer, "lr_scheduler": {"scheduler": lr_scheduler, "interval": "step"}}

@@ -22,6 +22,7 @@ Reference semantics followed (file:line of seas2nada/DPHuBERT):
 import contextlib
 import math
 import os
+import types
 from typing import List, Optional, Sequence
 
 import torch
@@ -246,6 +247,21 @@ def f32_cat(*ts: torch.Tensor) -> torch.Tensor:
     if all(t.requires_grad for t in ts):
         _CAT_REFRESH[id(out)] = (owner, ts, out)
     return out
+
+
+def i8_image(*ts: torch.Tensor) -> "K.I8Rows":
+    """Weights (concatenated along dim 0) as 8-bit integers with one scale an output channel (kernels.quant_rows_i8),
+    cached on the first one like bf16_image."""
+    owner = ts[0]
+    key = ("i8",) + _version_key(ts)
+    hit = getattr(owner, "_dph_i8", None)
+    if hit is not None and hit[0] == key:
+        return hit[1]
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("8-bit weights changed inside a HIP graph capture: run the model once before it")
+    w = ts[0].detach() if len(ts) == 1 else torch.cat([t.detach() for t in ts])
+    owner._dph_i8 = (key, K.quant_rows_i8(w))
+    return owner._dph_i8[1]
 
 
 def pad8(n: int) -> int:
@@ -2173,6 +2189,45 @@ class EncoderLayerFn(torch.autograd.Function):
 # ---------------------------------------------------------------------------
 # Distill projections + DistillLoss (fused)
 # ---------------------------------------------------------------------------
+@torch.no_grad()
+def encoder_layer_int8(cfg, h, layer, wl=None):
+    """An encoder layer's forward with its projections in 8-bit integers (kernels.linear_i8): h (B*T, D) -> the layer's
+    output, as EncoderLayerFn in eval mode (post-norm: bf16; pre-norm: the fp32 residual stream).  The LayerNorms in front
+    of a product quantise its tokens as they normalise them (kernels.layernorm_linear_i8); attention, biases and the
+    residual stream are the bf16 / fp32 path's.  layer: wav2vec2.components.EncoderLayer; wl: the WavLM bias tensors."""
+    w, att, ff = layer.int8_weights(), layer.attention, layer.feed_forward
+    ln1, ln2 = layer.layer_norm, layer.final_layer_norm
+    pre = cfg["pre_norm"]
+    if h.dtype != (F32 if pre else BF16):
+        raise ValueError(f"encoder layer input: expected {F32 if pre else BF16}, got {h.dtype}")
+    M, D = h.shape
+    dev = h.device
+    s1 = h
+    if att is not None:
+        bqkv = f32_cat(att.q_proj.bias, att.k_proj.bias, att.v_proj.bias)
+        if pre:
+            qkv, x_att = K.layernorm_linear_i8(h, ln1.weight, ln1.bias, w["qkv"], bqkv, eps=1e-5,
+                                               keep_norm=wl is not None)
+        else:
+            qkv, x_att = K.linear_i8(h, w["qkv"], bqkv), h
+        o_m = torch.empty(M, att.q_proj.weight.shape[0], dtype=BF16, device=dev)
+        EncoderLayerFn._attention_fwd(types.SimpleNamespace(wl=wl), cfg, x_att, qkv, None, o_m, None, None, 0)
+        s1 = K.linear_i8(o_m, w["out"], att.out_proj.bias, residual=h)
+    if pre:
+        if ff is None:
+            return s1.clone() if s1 is h else s1
+        f, _ = K.layernorm_linear_i8(s1, ln2.weight, ln2.bias, w["up"], ff.intermediate_dense.bias, act=K.ACT_GELU,
+                                     eps=1e-5)
+        return K.linear_i8(f, w["down"], ff.output_dense.bias, residual=s1)
+    if ff is not None:
+        f, h1 = K.layernorm_linear_i8(s1, ln1.weight, ln1.bias, w["up"], ff.intermediate_dense.bias, act=K.ACT_GELU,
+                                      eps=1e-5, keep_norm=True)
+        s2 = K.linear_i8(f, w["down"], ff.output_dense.bias, residual=h1)
+    else:
+        s2 = LayerNormFn.apply(s1, ln1.weight, ln1.bias)
+    return LayerNormFn.apply(s2, ln2.weight, ln2.bias)
+
+
 def _bf16_rows(xs):
     """bf16 copies of the fp32 tensors of ``xs`` (one per distinct tensor; bf16 ones pass through)."""
     done = {}

@@ -14,7 +14,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from ._lib import DphAdamGroup, DphTensorSlot, call, ptr
+from ._lib import DphAdamGroup, DphMuonSlot, DphTensorSlot, call, ptr
 
 CHUNK = 8192   # must match optim.hip
 SUMSQ_FLOATS = 1025   # DPH_SUMSQ_FLOATS (include/dphubert_hip.h)
@@ -64,6 +64,10 @@ class FusedAdamW(torch.optim.Optimizer):
         self._sumsq = torch.zeros(SUMSQ_FLOATS, dtype=torch.float32, device=dev)   # [0] = ||g||^2, [1:] partials
         self._chunk_key = key
 
+    def _state_keys(self, gi):
+        """The state tensors of a parameter of group ``gi``."""
+        return ("exp_avg", "exp_avg_sq")
+
     def _slot_table(self, plist):
         """Upload the (param, grad, exp_avg, exp_avg_sq) pointer table when any pointer changed.
         With a GradReducer the gradients are fixed bucket views, so this runs once."""
@@ -71,8 +75,8 @@ class FusedAdamW(torch.optim.Optimizer):
         for gi, p in plist:
             st = self.state[p]
             if len(st) == 0:
-                st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-                st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                for k in self._state_keys(gi):
+                    st[k] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 st["step"] = self._step_t
             elif st.get("step") is not self._step_t:
                 # loaded state (load_state_dict): adopt its step count, then share one counter
@@ -83,8 +87,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 p.grad = p.grad.contiguous()
             if p.grad is not None and p.grad.dtype != torch.float32:
                 raise TypeError("FusedAdamW expects fp32 gradients")
-            key.append((p.data_ptr(), p.grad.data_ptr() if p.grad is not None else 0, st["exp_avg"].data_ptr(),
-                        st["exp_avg_sq"].data_ptr(), p.numel(), gi))
+            ma, va = [st[k].data_ptr() for k in self._state_keys(gi)] + [0] * (2 - len(self._state_keys(gi)))
+            key.append((p.data_ptr(), p.grad.data_ptr() if p.grad is not None else 0, ma, va, p.numel(), gi))
         key = tuple(key)
         if key == self._slot_key:
             return
@@ -141,15 +145,19 @@ class FusedAdamW(torch.optim.Optimizer):
                 groups[gi].eps = g["eps"]
         from .kernels import SPAN_HINT
         SPAN_HINT["adamw_params"] = sum(p.numel() for _, p in plist)   # bench.py's kernel table (bytes per launch)
-        call("dph_adamw_step_img", ptr(self._slots_dev), len(plist), ptr(self._cslot), ptr(self._cstart),
-             self._nchunks, self.dyn_ptr, groups, len(self.param_groups), self._step,
-             ptr(self._sumsq) if clip else None, float(self.max_grad_norm or 0.0), ptr(img), s)
+        self._update(plist, dst, img, groups, clip, s)
         # the kernel wrote the masters behind autograd's back: bump their version counters so every
         # cached bf16 GEMM image of them (ops.bf16_image & co.) is rebuilt before its next use
         increment_version([p for _, p in plist])
         # cast the images the kernel did not cover, re-transpose the W^T images, and move the cache keys to the
         # new versions
         ops.refresh_images(ids, cast_done)
+
+    def _update(self, plist, dst, img, groups, clip, s):
+        """The update's launches, every parameter's bf16 image (``dst``) with it."""
+        call("dph_adamw_step_img", ptr(self._slots_dev), len(plist), ptr(self._cslot), ptr(self._cstart),
+             self._nchunks, self.dyn_ptr, groups, len(self.param_groups), self._step,
+             ptr(self._sumsq) if clip else None, float(self.max_grad_norm or 0.0), ptr(img), s)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -167,6 +175,105 @@ class FusedAdamW(torch.optim.Optimizer):
 import ctypes as _C  # noqa: E402
 
 C_SIZEOF_SLOT = _C.sizeof(DphTensorSlot)
+
+
+class FusedMuon(FusedAdamW):
+    """FusedAdamW whose groups marked ``muon=True`` take the Muon step instead: matrices (parameters of two dimensions, or
+    more taken as [first, rest]) move along the orthogonal factor of their momentum (kernels.newton_schulz),
+
+        m <- m + (g - m) (1 - beta),   u = g + (m - g) beta   (``nesterov``; else u = m)
+        p <- p (1 - lr weight_decay) - lr 0.2 sqrt(max(rows, columns)) orth(u)
+
+    with beta the group's ``momentum``.  orth(u)'s entries have the root mean square 1 / sqrt(max(rows, columns)), so a
+    step has 0.2 lr, about AdamW's, and AdamW's learning rates and weight decay carry over.  The gradient norm that
+    ``max_grad_norm`` clips is that of all groups.  State: ``momentum_buffer``; a parameter without a gradient is left
+    alone.  Captured in a HIP graph like FusedAdamW; the updates, their factors and the iteration's workspace are the
+    optimiser's own."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 max_grad_norm: Optional[float] = None, momentum: float = 0.95, nesterov: bool = True,
+                 ns_steps: int = 5, ns_coeffs=None, ns_eps: float = 1e-7):
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"momentum must be in [0, 1), got {momentum}")
+        if not 1 <= int(ns_steps) <= 64:
+            raise ValueError(f"ns_steps must be 1 to 64, got {ns_steps}")
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_grad_norm=max_grad_norm)
+        for g in self.param_groups:
+            if not g.get("muon", False):
+                continue
+            for p in g["params"]:
+                if p.dim() < 2 or p.numel() == 0:
+                    raise ValueError(f"muon group: parameters of two or more dimensions, got {tuple(p.shape)}")
+                if p.dtype != torch.float32 or not p.is_contiguous():
+                    raise ValueError("muon group: contiguous fp32 parameters")
+            g["momentum"] = g.get("momentum", momentum)
+            # (the kernels' beta1; also what StepScalars uploads)
+            g["betas"] = (g["momentum"], 0.0)
+        self.nesterov = bool(nesterov)
+        self._ns = dict(steps=int(ns_steps), eps=float(ns_eps))
+        if ns_coeffs is not None:
+            self._ns["coeffs"] = tuple(ns_coeffs)
+        self._muon_key = None
+
+    def _is_muon(self, gi):
+        return bool(self.param_groups[gi].get("muon", False))
+
+    def _state_keys(self, gi):
+        return ("momentum_buffer",) if self._is_muon(gi) else super()._state_keys(gi)
+
+    def _muon_tables(self, plist, dst):
+        """Slots, chunks, update buffers and the iteration's plan (rebuilt when a pointer moves)."""
+        at = [(i, gi, p) for i, (gi, p) in enumerate(plist) if self._is_muon(gi)]
+        key = tuple((p.data_ptr(), p.grad.data_ptr() if p.grad is not None else 0,
+                     self.state[p]["momentum_buffer"].data_ptr(), dst.get(id(p), 0), p.numel(), gi) for _, gi, p in at)
+        if key == self._muon_key:
+            return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedMuon: parameter/gradient storage changed inside a HIP graph capture")
+        from . import kernels as K
+        shapes = tuple((tuple(p.shape), p.device) for _, _, p in at)
+        if at and getattr(self, "_muon_shapes", None) != shapes:
+            dev = at[0][2].device
+            pad = lambda n: (n + 3) & ~3  # noqa: E731
+            flat = torch.zeros(sum(pad(p.numel()) for _, _, p in at), dtype=torch.float32, device=dev)
+            ups, o = [], 0
+            for _, _, p in at:
+                ups.append(flat[o:o + p.numel()].view(p.shape[0], -1))
+                o += pad(p.numel())
+            self._plan = K.NewtonSchulzPlan(ups, **self._ns)
+            cslot = [k for k, (_, _, p) in enumerate(at) for _ in range(0, p.numel(), CHUNK)]
+            cstart = [c for _, _, p in at for c in range(0, p.numel(), CHUNK)]
+            self._m_cslot = torch.tensor(cslot, dtype=torch.int64, device=dev)
+            self._m_cstart = torch.tensor(cstart, dtype=torch.int64, device=dev)
+            rest = [(i, c) for i, (gi, p) in enumerate(plist) if not self._is_muon(gi)
+                    for c in range(0, p.numel(), CHUNK)]
+            self._a_cslot = torch.tensor([i for i, _ in rest], dtype=torch.int64, device=dev)
+            self._a_cstart = torch.tensor([c for _, c in rest], dtype=torch.int64, device=dev)
+            self._muon_shapes = shapes
+        if at:
+            slots = (DphMuonSlot * len(at))()
+            for s, k, u, o, (_, _, p) in zip(slots, key, self._plan.mats, self._plan.out, at):
+                s.param, s.grad, s.momentum, s.img, s.n, s.group = k
+                s.update, s.dir = u.data_ptr(), o.data_ptr()
+                s.scale = 0.2 * math.sqrt(max(u.shape))
+            # (a synchronous copy: pointers move when buffers are first laid out, not from step to step)
+            host = torch.frombuffer(bytearray(bytes(slots)), dtype=torch.uint8)
+            self._m_slots = host.to(at[0][2].device)
+        self._muon_key = key
+
+    def _update(self, plist, dst, img, groups, clip, s):
+        self._muon_tables(plist, dst)
+        if not self._muon_key:
+            return super()._update(plist, dst, img, groups, clip, s)
+        ng, sumsq, mx = len(self.param_groups), ptr(self._sumsq) if clip else None, float(self.max_grad_norm or 0.0)
+        if self._a_cslot.numel():
+            call("dph_adamw_step_img", ptr(self._slots_dev), len(plist), ptr(self._a_cslot), ptr(self._a_cstart),
+                 self._a_cslot.numel(), self.dyn_ptr, groups, ng, self._step, sumsq, mx, ptr(img), s)
+        m = (ptr(self._m_slots), len(self._muon_key), ptr(self._m_cslot), ptr(self._m_cstart), self._m_cslot.numel(),
+             self.dyn_ptr, groups, ng)
+        call("dph_muon_momentum", *m, int(self.nesterov), sumsq, mx, s)
+        self._plan.run()
+        call("dph_muon_apply", *m, s)
 
 
 class LinearDecayLRScheduler(torch.optim.lr_scheduler.LRScheduler):

@@ -72,7 +72,8 @@ def build_distill_module(teacher_config: dict, student_config: Optional[dict] = 
                          cos_type: str = "raw", learning_rate: float = 2e-4, weight_decay: float = 0.0,
                          warmup_updates: int = 15000, max_updates: int = 50000, reg_learning_rate: float = 0.02,
                          target_sparsity: float = 0.75, sparsity_warmup_updates: int = 5000,
-                         proj_state: Optional[dict] = None) -> DistillModule:
+                         proj_state: Optional[dict] = None, optimizer: str = "adamw",
+                         muon_momentum: float = 0.95) -> DistillModule:
     teacher = wav2vec2_model(**copy.deepcopy(teacher_config))
     if teacher_state is not None:
         teacher.load_state_dict(teacher_state, strict=False)
@@ -103,7 +104,8 @@ def build_distill_module(teacher_config: dict, student_config: Optional[dict] = 
                          max_updates=max_updates, use_reg=use_reg,
                          reg_learning_rate=reg_learning_rate if use_reg else None,
                          target_sparsity=target_sparsity if use_reg else None,
-                         sparsity_warmup_updates=sparsity_warmup_updates if use_reg else None)
+                         sparsity_warmup_updates=sparsity_warmup_updates if use_reg else None, optimizer=optimizer,
+                         muon_momentum=muon_momentum)
 
 
 def fused_grad_groups(model) -> List[tuple]:

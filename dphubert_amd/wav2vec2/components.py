@@ -480,6 +480,31 @@ class EncoderLayer(Module):
         self.feed_forward = feed_forward
         self.final_layer_norm = nn.LayerNorm(embed_dim)
         self.embed_dim = embed_dim
+        self.int8 = False            # Wav2Vec2Model.quantize_int8
+
+    def check_int8(self):
+        """Raise unless the layer can run in 8-bit integers (ops.encoder_layer_int8)."""
+        from .._lib import I8_LN_MAX
+        for m in (self.attention, self.feed_forward):
+            gates = [n for n, c in m.named_children() if isinstance(c, HardConcrete)] if m is not None else []
+            if gates:
+                raise ValueError(f"quantize_int8: the layer still has pruning gates ({', '.join(gates)}): prune() first")
+        if self.embed_dim > I8_LN_MAX:
+            raise ValueError(f"quantize_int8: embed_dim up to {I8_LN_MAX}, got {self.embed_dim}")
+        if not next(self.parameters()).is_cuda:
+            raise ValueError("quantize_int8 runs on the HIP path only: move the model to the device first")
+
+    def int8_weights(self):
+        """The layer's weights as 8-bit integers (cached per parameter version): ops.i8_image."""
+        a, f = self.attention, self.feed_forward
+        w = {}
+        if a is not None:
+            w["qkv"] = ops.i8_image(a.q_proj.weight, a.k_proj.weight, a.v_proj.weight)
+            w["out"] = ops.i8_image(a.out_proj.weight)
+        if f is not None:
+            w["up"] = ops.i8_image(f.intermediate_dense.weight)
+            w["down"] = ops.i8_image(f.output_dense.weight)
+        return w
 
     def forward(self, x: Tensor, attention_mask=None, position_bias: Optional[Tensor] = None,
                 key_padding_mask: Optional[Tensor] = None, key_len: Optional[Tensor] = None):
@@ -524,6 +549,13 @@ class EncoderLayer(Module):
                 gw, gb, gc = att.gru_rel_pos_linear.weight, att.gru_rel_pos_linear.bias, att.gru_rel_pos_const
                 cfg["wavlm"] = True
         a = att
+        if self.int8:
+            if need or tr:
+                raise RuntimeError("an encoder layer in 8-bit integers is forward only: eval mode without gradients "
+                                   "(quantize_int8(False) goes back to bf16)")
+            wl = dict(rel_tab=rel_tab, gw=gw, gb=gb, gc=gc, heads=heads) if rel_tab is not None else None
+            out = ops.encoder_layer_int8(cfg, x.reshape(B * T, D), self, wl)
+            return out.view(B, T, D), position_bias
         out = ops.EncoderLayerFn.apply(
             cfg, x.reshape(B * T, D),
             a.q_proj.weight if a else None, a.k_proj.weight if a else None, a.v_proj.weight if a else None,

@@ -130,6 +130,22 @@ class Wav2Vec2Model(Module):
             return torch.tensor(float(self._np_table.constant), device=next(self.parameters()).device)
         return ops.ExpectedParamsFn.apply(self._np_table, *las)
 
+    def quantize_int8(self, enable: bool = True):
+        """Run the encoder layers' projections (query / key / value, output, both feed-forward ones) in 8-bit integers:
+        weights with one scale an output channel, laid out now and again whenever they change, activations with one
+        scale a token.  Forward only -- eval mode, no gradients: a frozen teacher, inference of a pruned student.  The
+        rest of the model, and the hidden states' types, stay as they are.  ``enable=False`` goes back to bf16."""
+        layers = self.encoder.transformer.layers
+        if enable:
+            for layer in layers:
+                layer.check_int8()
+            self.eval()
+        for layer in layers:
+            layer.int8 = bool(enable)
+            if enable:
+                layer.int8_weights()
+        return self
+
     def prune(self):
         """Eval-mode structural pruning (model.py:115-125)."""
         self.eval()

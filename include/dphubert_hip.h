@@ -703,6 +703,29 @@ int64_t dph_newton_schulz_workspace(const DphNsGroup* groups, int64_t n_groups);
 int dph_newton_schulz(const DphNsMat* mats, const DphNsGroup* groups, int64_t n_groups, int64_t steps,
                       const float* coeffs, float eps, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
+/* Muon (ABI 25): the update of a matrix is the orthogonal factor of its momentum.  One slot a parameter; chunk tables,
+ * dyn / groups, sumsq and max_norm as dph_adamw_step_img.  A slot without a gradient is left alone.
+ * dph_muon_momentum: g = grad * clip (written back where it was clipped), momentum += (g - momentum) (1 - beta1), and
+ * update = g + (momentum - g) beta1 (nesterov != 0) or momentum: what dph_newton_schulz takes.
+ * dph_muon_apply: param = param (1 - lr weight_decay) - lr scale dir, cast to img (bf16) too where that is given. */
+typedef struct DphMuonSlot {
+  float* param;
+  float* grad;
+  float* momentum;
+  float* update;
+  const uint16_t* dir; /* bf16, as param */
+  uint16_t* img;       /* NULL: none */
+  int64_t n;
+  float scale;
+  int32_t group;
+} DphMuonSlot;
+int dph_muon_momentum(const DphMuonSlot* slots, int64_t n_slots, const int64_t* chunk_slot, const int64_t* chunk_start,
+                      int64_t n_chunks, const DphAdamDyn* dyn, const DphAdamGroup* groups, int64_t n_groups,
+                      int nesterov, const float* sumsq, float max_norm, hipStream_t stream);
+int dph_muon_apply(const DphMuonSlot* slots, int64_t n_slots, const int64_t* chunk_slot, const int64_t* chunk_start,
+                   int64_t n_chunks, const DphAdamDyn* dyn, const DphAdamGroup* groups, int64_t n_groups,
+                   hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
