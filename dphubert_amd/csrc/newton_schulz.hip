@@ -41,6 +41,10 @@ constexpr int NS_MATS = 64;        // matrices of one packing launch
 constexpr float NS_E = 64.f;       // E and F are held times 64 (entries of a few 1e-5 stay normal fp16 numbers)
 constexpr int NS_PARTS = 64;       // partial sums of a matrix's squares
 constexpr int NS_SPLIT = 128;      // rows up to which all operands are held in two parts
+// The Gram matrix of few rows and many columns is few tiles and a long sum: up to NS_DEEP rows, from NS_LONG columns on,
+// the sum is cut into parts of a fixed number of steps (by the shape alone, so that a result does not depend on what else
+// is in the list), whose tiles are added in their order by a launch of their own.  4 matrices of 128 x 4000: 617 -> 195 us.
+constexpr int NS_DEEP = 256, NS_LONG = 1024;
 
 __device__ __forceinline__ f16_t f2h(float v) { return __builtin_bit_cast(f16_t, (_Float16)v); }
 __device__ __forceinline__ float h2f(f16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
@@ -84,6 +88,8 @@ struct Group {
   char *e, *f, *el, *fl;              // [cnt][mp][mp]; the lower halves (split) or null
   double* part;                       // [cnt][NS_PARTS]
   bf16_t* out;                        // [cnt] matrices as the caller has them, dense
+  float* slab;                        // [cnt][tiles of the Gram matrix][parts][64 x 64] sums
+  int32_t parts, part_steps;          // of the Gram matrix's sum (1: none)
 };
 struct Groups {
   int32_t ng;
@@ -244,7 +250,8 @@ __device__ __forceinline__ uint2 quad_transpose(uint2 x, int lane) {
   return o2 ? make_uint2(b1, a1) : make_uint2(a0, b0);
 }
 
-template <int KIND, bool SPLIT, class C>
+// FINISH: the Gram matrix's parts are added, and no product is made
+template <int KIND, bool SPLIT, class C, bool FINISH>
 __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups gs, const Step st) {
   __shared__ __align__(16) char smem[C::LDS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -257,10 +264,19 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
   t -= gs.first[k];
   constexpr bool SYM = KIND == GRAM || KIND == POLY;
   using T = std::conditional_t<KIND == GRAM, mt::F16T, mt::F16>;
-  int ti, tj, z;
+  int ti, tj, z, kp = 0;
+  float* slab = nullptr;
+  constexpr bool PARTS = KIND == GRAM && C::BM == 64 && C::BN == 64;
   if (SYM) {
     static_assert(!SYM || C::BM == C::BN, "square tiles");
     const int tm = (g.m + C::BM - 1) / C::BM, per = tm * (tm + 1) / 2;
+    if (PARTS && g.parts > 1) {
+      slab = g.slab + (int64_t)t * (FINISH ? g.parts : 1) * 4096;
+      if (!FINISH) {
+        kp = t % g.parts;
+        t /= g.parts;
+      }
+    }
     z = t / per;
     t -= z * per;
     ti = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
@@ -276,8 +292,13 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
   }
   const int m0 = ti * C::BM, n0 = tj * C::BN;
   const int64_t yoff = (int64_t)z * g.np * g.mp * 2, eoff = (int64_t)z * g.mp * g.mp * 2;
-  const int kbytes = (KIND == GRAM ? g.np : g.mp) * 2;
+  int kbytes = (KIND == GRAM ? g.np : g.mp) * 2;
   const int64_t ld = (int64_t)g.mp * 2;
+  int64_t koff = 0;                   // bytes of the part's first k-row
+  if (PARTS && slab) {
+    koff = (int64_t)kp * g.part_steps * 64 * ld;
+    kbytes = min(g.part_steps * 128, kbytes - kp * g.part_steps * 128);
+  }
   using V = mt::Strip<C::FN, C::FN % 4 == 0 ? NSW : 8>;
   constexpr int NV = 4 * C::FN;
   f32x4_t acc[C::FM][C::FN];
@@ -326,13 +347,22 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
       }
     }
   };
+  const auto at = [&](int i, int j) { return ((wave * C::FM + i) * C::FN + j) * 256 + lane * 4; };   // in a part's tile
+  if constexpr (FINISH) {
+    init();
+    for (int p = 0; p < g.parts; ++p)
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < C::FN; ++j) acc[i][j] += *reinterpret_cast<const f32x4_t*>(slab + (int64_t)p * 4096 + at(i, j));
+  }
 #pragma unroll 1
-  for (int part = 0; part < (SPLIT ? 3 : 1); ++part) {   // h h, l h, h l
+  for (int part = 0; part < (FINISH ? 0 : SPLIT ? 3 : 1); ++part) {   // h h, l h, h l
     const bool la = part == 1, lb = part == 2;
     mt::Rows A, B;
     if constexpr (KIND == GRAM) {
-      A = mt::Rows{(la ? g.yl[st.cur] : g.y[st.cur]) + yoff, ld, g.mp};
-      B = mt::Rows{(lb ? g.yl[st.cur] : g.y[st.cur]) + yoff, ld, g.mp};
+      A = mt::Rows{(la ? g.yl[st.cur] : g.y[st.cur]) + yoff + koff, ld, g.mp};
+      B = mt::Rows{(lb ? g.yl[st.cur] : g.y[st.cur]) + yoff + koff, ld, g.mp};
     } else if constexpr (KIND == POLY) {
       A = mt::Rows{(la ? g.el : g.e) + eoff, ld, g.mp};
       B = mt::Rows{(lb ? g.el : g.e) + eoff, ld, g.mp};
@@ -343,6 +373,13 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
     mt::product_of<T, C>(A, B, kbytes, m0, n0, acc, smem, wave, lane, [&]() {
       if (!SPLIT || part == 0) init();
     });
+  }
+  if (PARTS && !FINISH && slab) {
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) *reinterpret_cast<f32x4_t*>(slab + at(i, j)) = acc[i][j];
+    return;
   }
 
 #pragma unroll
@@ -462,6 +499,10 @@ int64_t group_bytes(const DphNsGroup& g, char* at, Group* out) {
   const int64_t mp = up64(m), np = up64(n), y = g.count * np * mp * 2, e = g.count * mp * mp * 2;
   const int64_t part = g.count * NS_PARTS * (int64_t)sizeof(double);
   const bool split = m <= NS_SPLIT;
+  // parts of at least 4 steps of 64 columns, 32 at most
+  const int64_t steps = np / 64, want = m <= NS_DEEP && n >= NS_LONG ? (steps / 4 < 32 ? steps / 4 : 32) : 1;
+  const int64_t part_steps = cdiv(steps, want), parts = cdiv(steps, part_steps), tm = mp / 64;
+  const int64_t slab = parts > 1 ? g.count * (tm * (tm + 1) / 2) * parts * 4096 * (int64_t)sizeof(float) : 0;
   if (out) {
     out->part = reinterpret_cast<double*>(at);
     at += part;
@@ -479,8 +520,11 @@ int64_t group_bytes(const DphNsGroup& g, char* at, Group* out) {
     out->yl[1] = take(split, y);
     out->el = take(split, e);
     out->fl = take(split, e);
+    out->slab = reinterpret_cast<float*>(take(slab > 0, slab));
+    out->parts = (int32_t)parts;
+    out->part_steps = (int32_t)part_steps;
   }
-  return part + 2 * y + 2 * e + (split ? 2 * y + 2 * e : y / 2);
+  return part + 2 * y + 2 * e + (split ? 2 * y + 2 * e : y / 2) + slab;
 }
 
 int check_groups(const DphNsGroup* groups, int64_t n, const char* who) {
@@ -513,29 +557,33 @@ extern "C" int64_t dph_newton_schulz_workspace(const DphNsGroup* groups, int64_t
 namespace dph {
 namespace {
 
-// the groups whose operands are split, or the others, and their tiles of C
-template <int KIND, bool SPLIT, class C>
-int64_t choose(const Groups& all, Groups* gs) {
+// Kinds of groups: operands split or not, the Gram matrix's sum in parts or not
+enum { SHALLOW = 1, DEEP = 2 };
+
+// the groups that are split, or the others, of these kinds, and how many workgroups their tiles of C take
+template <int KIND, bool SPLIT, class C, bool FINISH>
+int64_t choose(const Groups& all, int kinds, Groups* gs) {
   int64_t tiles = 0;
   gs->ng = 0;
   for (int i = 0; i < all.ng; ++i) {
     const Group& g = all.g[i];
-    if ((g.el != nullptr) != SPLIT) continue;
+    if ((g.el != nullptr) != SPLIT || !(kinds & (g.parts > 1 ? DEEP : SHALLOW))) continue;
     const int64_t tm = cdiv(g.m, C::BN), tn = cdiv(g.n, C::BM);
     gs->first[gs->ng] = (int32_t)tiles;
     gs->g[gs->ng++] = g;
-    tiles += (KIND == GRAM || KIND == POLY ? tm * (tm + 1) / 2 : tm * tn) * g.cnt;
+    tiles += (KIND == GRAM || KIND == POLY ? tm * (tm + 1) / 2 : tm * tn) * g.cnt *
+             (KIND == GRAM && C::BM == 64 && !FINISH ? g.parts : 1);
     if (tiles >= (1 << 22)) return -1;
   }
   return tiles;
 }
-template <int KIND, bool SPLIT, class C>
-int launch_tiles(const Groups& all, const Step& st, hipStream_t stream) {
+template <int KIND, bool SPLIT, class C, bool FINISH = false>
+int launch_tiles(const Groups& all, int kinds, const Step& st, hipStream_t stream) {
   Groups gs = {};
-  const int64_t tiles = choose<KIND, SPLIT, C>(all, &gs);
+  const int64_t tiles = choose<KIND, SPLIT, C, FINISH>(all, kinds, &gs);
   DPH_REQUIRE(tiles >= 0, "dph_newton_schulz: too many tiles");
   if (tiles == 0) return DPH_OK;
-  hipLaunchKernelGGL((ns_product_kernel<KIND, SPLIT, C>), dim3((unsigned)tiles), dim3(C::NT), 0, stream, gs, st);
+  hipLaunchKernelGGL((ns_product_kernel<KIND, SPLIT, C, FINISH>), dim3((unsigned)tiles), dim3(C::NT), 0, stream, gs, st);
   return check_launch("dph_newton_schulz");
 }
 
@@ -543,14 +591,22 @@ int launch_tiles(const Groups& all, const Step& st, hipStream_t stream) {
 // 768 1.11 / 0.88 / 1.20 ms, one of 768 x 768 472 / 221 / 147 us, 8 of 448 x 768 396 / 188 / 152 us.
 template <int KIND>
 int launch_product(const Groups& gs, const Step& st, hipStream_t stream) {
-  DPH_TRY((launch_tiles<KIND, true, mt::C64>(gs, st, stream)));
+  // (sums in parts: tiles of 64 x 64 only)
+  const int any = KIND == GRAM ? SHALLOW : SHALLOW | DEEP;
+  DPH_TRY((launch_tiles<KIND, true, mt::C64>(gs, SHALLOW | DEEP, st, stream)));
+  if constexpr (KIND == GRAM) {
+    DPH_TRY((launch_tiles<KIND, false, mt::C64>(gs, DEEP, st, stream)));
+    DPH_TRY((launch_tiles<KIND, true, mt::C64, true>(gs, DEEP, st, stream)));
+    DPH_TRY((launch_tiles<KIND, false, mt::C64, true>(gs, DEEP, st, stream)));
+  }
   Groups some = {};
-  const int64_t t256 = choose<KIND, false, mt::C256>(gs, &some), t128 = choose<KIND, false, mt::C128>(gs, &some),
-                t64 = choose<KIND, false, mt::C64>(gs, &some);
+  const int64_t t256 = choose<KIND, false, mt::C256, false>(gs, any, &some),
+                t128 = choose<KIND, false, mt::C128, false>(gs, any, &some),
+                t64 = choose<KIND, false, mt::C64, false>(gs, any, &some);
   const int tile = t256 < 0 ? 256 : mt::choose_tile(t256, t128, t64);
-  if (tile == 64) return launch_tiles<KIND, false, mt::C64>(gs, st, stream);
-  if (tile == 128) return launch_tiles<KIND, false, mt::C128>(gs, st, stream);
-  return launch_tiles<KIND, false, mt::C256>(gs, st, stream);
+  if (tile == 64) return launch_tiles<KIND, false, mt::C64>(gs, any, st, stream);
+  if (tile == 128) return launch_tiles<KIND, false, mt::C128>(gs, any, st, stream);
+  return launch_tiles<KIND, false, mt::C256>(gs, any, st, stream);
 }
 
 // up to NS_GROUPS groups, whose matrices start at mats

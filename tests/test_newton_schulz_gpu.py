@@ -55,7 +55,8 @@ def strong(m, n, g, dt=F32):
 
 
 SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (5, 3), (16, 64), (64, 16), (63, 65), (64, 64), (100, 100), (128, 128), (129, 127), (129, 400),
-          (257, 255), (384, 1000), (1000, 129), (512, 512), (300, 2047)]
+          (257, 255), (384, 1000), (1000, 129), (512, 512), (300, 2047),
+          (3, 1024), (1500, 64), (130, 1100), (100, 5000), (256, 9000), (20000, 5)]
 
 
 @pytest.mark.parametrize("dt", [BF16, F32])
