@@ -281,9 +281,14 @@ _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def stream_ptr(device=None) -> int:
-    if device is None and _RAW_STREAM is not None and torch.cuda.is_initialized():
-        return _RAW_STREAM(torch.cuda.current_device())
+    if device is None and torch.cuda.is_initialized():
+        return stream_of(torch.cuda.current_device())
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def stream_of(index: int) -> int:
+    """The current stream of device ``index`` of an initialised runtime."""
+    return _RAW_STREAM(index) if _RAW_STREAM is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def ptr(t):

@@ -492,49 +492,55 @@ class _on_device:
 
 
 def _chk_on(dev, t, name, dtypes, ndim):
+    """The shape of a device tensor of these types and dimensions on ``dev``."""
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.device == dev and dev.type == "cuda":
+        shape = t.shape
+        if len(shape) == ndim:
+            return shape
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor (no CPU path)")
     if t.device != dev:
         raise ValueError(f"{name} is on {t.device}, the input on {dev}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name}: expected {' or '.join(map(str, dtypes))}, got {t.dtype}")
-    if t.dim() != ndim:
-        raise ValueError(f"{name}: expected {ndim} dimensions, got shape {tuple(t.shape)}")
+    raise ValueError(f"{name}: expected {ndim} dimensions, got shape {tuple(t.shape)}")
 
 
-def _chk_rows(t, name):
+def _chk_rows(t, R, K, name):
     """[R, K] rows of unit stride that do not overlap; their distance in elements."""
-    R, K = t.shape
     ld, one = t.stride()
-    if K > 1 and one != 1:
+    if one != 1 and K > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous (strides {t.stride()})")
-    if R > 1:
-        if ld < K:
+    if ld < K:
+        if R > 1:
             raise ValueError(f"{name}: rows overlap (strides {t.stride()})")
-        return ld
-    return max(ld, K)
+        return K
+    return ld
 
 
 def _chk_vec(dev, t, name, n):
-    _chk_on(dev, t, name, (F32,), 1)
-    if t.shape[0] != n or not t.is_contiguous():
+    shape = _chk_on(dev, t, name, _F32_ONLY, 1)
+    if shape[0] != n or not t.is_contiguous():
         raise ValueError(f"{name}: expected {n} contiguous elements, got shape {tuple(t.shape)}, strides {t.stride()}")
 
 
 def _chk_i8(dev, r, name):
     """(rows, columns, the distance of the rows in bytes) of an I8Rows."""
     q, scale = r
-    _chk_on(dev, q, name + ".q", (torch.int8,), 2)
-    R, K = q.shape
-    _chk_vec(dev, scale, name + ".scale", R)
-    ld = _chk_rows(q, name + ".q")
+    R, K = _chk_on(dev, q, name, _I8_ONLY, 2)
+    _chk_vec(dev, scale, name, R)
+    ld = _chk_rows(q, R, K, name)
     if R == 1:
         ld = _i8_ld(K)
+    # (only where a row ends inside 16 bytes is anything read behind the last one)
     if R and (ld % 16 or q.data_ptr() % 16 or
-              q.storage_offset() + (R - 1) * ld + _i8_ld(K) > q.untyped_storage().nbytes()):
+              (K % 16 and q.storage_offset() + (R - 1) * ld + _i8_ld(K) > q.untyped_storage().nbytes())):
         raise ValueError(f"{name}.q: rows must start (and be readable to) a multiple of 16 bytes, as quant_rows_i8 lays "
                          f"them out; shape {tuple(q.shape)}, strides {q.stride()}")
     return R, K, ld
+
+
+_F32_ONLY, _I8_ONLY, _FLOATS = (F32,), (torch.int8,), (BF16, F32)
 
 
 def _i8_ld(K: int) -> int:
@@ -548,11 +554,10 @@ def quant_rows_i8(x: torch.Tensor) -> I8Rows:
     apart (row-strided views)."""
     if not isinstance(x, torch.Tensor):
         raise ValueError("x must be a device tensor (no CPU path)")
-    _chk_on(x.device, x, "x", (BF16, F32), 2)
-    R, K = x.shape
+    R, K = _chk_on(x.device, x, "x", _FLOATS, 2)
     if not 1 <= K <= _lib.I8_K_MAX:
         raise ValueError(f"x: rows of 1 to {_lib.I8_K_MAX} elements, got {K}")
-    ldx = _chk_rows(x, "x")
+    ldx = _chk_rows(x, R, K, "x")
     ld = _i8_ld(K)
     with _on_device(x.device):
         q = torch.empty(R, ld, dtype=torch.int8, device=x.device)
@@ -567,6 +572,7 @@ assert _I8_ARGS.size == C.sizeof(_lib.DphLinearI8Args)
 
 
 def _linear_i8(x, w, bias, act, residual, out, out_dtype, ln, keep_norm):
+    # (a call of a few rows takes as long as the host needs for it: one look at each attribute)
     rows = isinstance(x, I8Rows)
     t = x.q if rows else x
     if not isinstance(t, torch.Tensor):
@@ -578,61 +584,53 @@ def _linear_i8(x, w, bias, act, residual, out, out_dtype, ln, keep_norm):
     if rows:
         M, Kx, ldq = _chk_i8(dev, x, "x")
     else:
-        _chk_on(dev, x, "x", (BF16, F32), 2)
-        M, Kx = x.shape
-        ldx = _chk_rows(x, "x")
+        M, Kx = _chk_on(dev, x, "x", _FLOATS, 2)
+        ldx = _chk_rows(x, M, Kx, "x")
     if Kx != K:
         raise ValueError(f"x has rows of {Kx} elements, w of {K}")
     if not 1 <= K <= _lib.I8_K_MAX:
         raise ValueError(f"x: rows of 1 to {_lib.I8_K_MAX} elements, got {K}")
-    if act not in (ACT_NONE, ACT_GELU):
+    if act != ACT_NONE and act != ACT_GELU:
         raise ValueError(f"act must be ACT_NONE or ACT_GELU, got {act}")
+    bp = rp = ldr = 0
     if bias is not None:
         _chk_vec(dev, bias, "bias", N)
-    ldr = 0
+        bp = bias.data_ptr()
     if residual is not None:
-        _chk_on(dev, residual, "residual", (BF16, F32), 2)
-        if residual.shape[0] != M or residual.shape[1] != N:
+        if tuple(_chk_on(dev, residual, "residual", _FLOATS, 2)) != (M, N):
             raise ValueError(f"residual: expected {(M, N)}, got {tuple(residual.shape)}")
         out_dtype = residual.dtype
-        ldr = _chk_rows(residual, "residual")
-    elif out_dtype not in (BF16, F32):
+        ldr, rp = _chk_rows(residual, M, N, "residual"), residual.data_ptr()
+    elif out_dtype not in _FLOATS:
         raise ValueError(f"out_dtype must be bf16 or fp32, got {out_dtype}")
-    norm = None
-    with _on_device(dev):
-        if out is None:
-            out = torch.empty((M, N), dtype=out_dtype, device=dev)
-            ldo = N
-        else:
-            _chk_on(dev, out, "out", (out_dtype,), 2)
-            if out.shape[0] != M or out.shape[1] != N:
-                raise ValueError(f"out: expected {(M, N)}, got {tuple(out.shape)}")
-            ldo = _chk_rows(out, "out")
-        if not M:
-            return out, torch.empty((0, K), dtype=BF16, device=dev) if keep_norm else None
-        if rows:
-            xp, xf, ldx = 0, 0, 0
-            qp, sp = x.q.data_ptr(), x.scale.data_ptr()
-        else:
-            xp, xf, ldq, qp, sp = x.data_ptr(), x.dtype == F32, _i8_ld(K), 0, 0
-            nbytes = _lib.lib().dph_linear_i8_workspace(M, N, K)
-            if nbytes:
-                ws = torch.empty(nbytes, dtype=torch.int8, device=dev)    # q, then the scales
-                qp = ws.data_ptr()
-                sp = qp + M * ldq
-        lw = lb = np = 0
-        eps = 0.0
-        if ln is not None:
-            lw, lb, eps = ln
-            if keep_norm:
-                norm = torch.empty((M, K), dtype=BF16, device=dev)
-                np = norm.data_ptr()
-        f32 = out_dtype == F32
-        call("dph_linear_i8",
-             _I8_ARGS.pack(M, N, K, xp, ldx, xf, act, lw, lb, np, K, qp, ldq, sp, w.q.data_ptr(), ldw,
-                           w.scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
-                           0 if residual is None else residual.data_ptr(), ldr, out.data_ptr(), ldo, f32,
-                           OUT_F32 if f32 else OUT_BF16, eps, 0), _stream())
+    f32 = out_dtype == F32
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _linear_i8(x, w, bias, act, residual, out, out_dtype, ln, keep_norm)
+    if out is None:
+        out, ldo = torch.empty((M, N), dtype=out_dtype, device=dev), N
+    else:
+        if tuple(_chk_on(dev, out, "out", (out_dtype,), 2)) != (M, N):
+            raise ValueError(f"out: expected {(M, N)}, got {tuple(out.shape)}")
+        ldo = _chk_rows(out, M, N, "out")
+    norm = torch.empty((M, K), dtype=BF16, device=dev) if keep_norm else None
+    if not M:
+        return out, norm
+    if rows:
+        xp, xf, ldx = 0, 0, 0
+        qp, sp = x.q.data_ptr(), x.scale.data_ptr()
+    else:
+        xp, xf, ldq, qp, sp = x.data_ptr(), x.dtype == F32, _i8_ld(K), 0, 0
+        nbytes = _lib.lib().dph_linear_i8_workspace(M, N, K)
+        if nbytes:
+            ws = torch.empty((nbytes,), dtype=torch.int8, device=dev)    # q, then the scales
+            qp = ws.data_ptr()
+            sp = qp + M * ldq
+    lw, lb, eps = ln or (0, 0, 0.0)
+    call("dph_linear_i8",
+         _I8_ARGS.pack(M, N, K, xp, ldx, xf, act, lw, lb, 0 if norm is None else norm.data_ptr(), K, qp, ldq, sp,
+                       w.q.data_ptr(), ldw, w.scale.data_ptr(), bp, rp, ldr, out.data_ptr(), ldo, f32,
+                       OUT_F32 if f32 else OUT_BF16, eps, 0), _lib.stream_of(dev.index))
     return out, norm
 
 
@@ -657,8 +655,7 @@ def layernorm_linear_i8(x: torch.Tensor, ln_weight: torch.Tensor, ln_bias: torch
     come from the values before their rounding to bf16.  The product is bf16."""
     if not isinstance(x, torch.Tensor):
         raise ValueError("x must be a device tensor (no CPU path)")
-    _chk_on(x.device, x, "x", (BF16, F32), 2)
-    K = x.shape[1]
+    K = _chk_on(x.device, x, "x", _FLOATS, 2)[1]
     if not 1 <= K <= _lib.I8_LN_MAX:
         raise ValueError(f"x: rows of 1 to {_lib.I8_LN_MAX} elements, got {K}")
     _chk_vec(x.device, ln_weight, "ln_weight", K)
@@ -682,7 +679,9 @@ class NewtonSchulzPlan:
         mats = list(mats)
         if not mats:
             raise ValueError("mats is empty")
-        dev = mats[0].device if isinstance(mats[0], torch.Tensor) else None
+        if not isinstance(mats[0], torch.Tensor):
+            raise ValueError("mats[0] must be a device tensor (no CPU path)")
+        dev = mats[0].device
         if not 1 <= int(steps) <= 64:
             raise ValueError(f"steps must be 1 to 64, got {steps}")
         if len(coeffs) != 3:
@@ -691,8 +690,7 @@ class NewtonSchulzPlan:
             raise ValueError(f"eps must not be negative, got {eps}")
         places = {}
         for i, t in enumerate(mats):
-            _chk_on(dev, t, f"mats[{i}]", (BF16, F32), 2)
-            R, K = t.shape
+            R, K = _chk_on(dev, t, f"mats[{i}]", _FLOATS, 2)
             if not (R and K):
                 raise ValueError(f"mats[{i}] is empty: {tuple(t.shape)}")
             s0, s1 = t.stride()
@@ -735,7 +733,8 @@ def newton_schulz(mats: Sequence[torch.Tensor], *, steps: int = 5, coeffs: Seque
 
     mats: 2-D tensors of one device, bf16 or fp32, of any shapes and row strides (a transposed view will do).  Returns
     bf16 tensors of the same shapes.  Matrices of all shapes share launches, so hand in a whole model's at once.  The
-    results are within about two bf16 roundings of the iteration in 64 bits (newton_schulz.hip)."""
+    results are within about two bf16 roundings of the iteration in 64 bits (newton_schulz.hip).  A zero matrix gives
+    zeros (eps > 0), one with an infinity or a NaN gives NaN; coefficients under which X's entries pass 4 overflow."""
     mats = list(mats)
     if not mats:
         if not 1 <= int(steps) <= 64:

@@ -253,7 +253,7 @@ def i8_image(*ts: torch.Tensor) -> "K.I8Rows":
     """Weights (concatenated along dim 0) as 8-bit integers with one scale an output channel (kernels.quant_rows_i8),
     cached on the first one like bf16_image."""
     owner = ts[0]
-    key = ("i8",) + _version_key(ts)
+    key = ("i8", owner.device) + _version_key(ts)
     hit = getattr(owner, "_dph_i8", None)
     if hit is not None and hit[0] == key:
         return hit[1]
