@@ -93,11 +93,12 @@ __device__ __forceinline__ uint2 pack8(const float (&v)[8], float inv, float s) 
 }
 
 // exact-erf GELU as common.h's (Abramowitz & Stegun 7.1.26, 1.5e-7), in the form max(x, 0) - |x| erfc(|x| / sqrt 2) / 2: no
-// comparison, and the halves and square roots are in the constants (58 -> 56 us at 7984 x 4096 x 1024, where it is a third)
+// comparison, and the halves and square roots are in the constants (58 -> 56 us at 7984 x 4096 x 1024, where it is a third).
+// An infinite |x| is cut off where it meets the erfc's zero (a NaN stays one: it comes through t)
 __device__ __forceinline__ float gelu_i8(float x) {
   const float ax = fabsf(x), t = __builtin_amdgcn_rcpf(fmaf(0.23164189f, ax, 1.0f));
   const float p = t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
-  return fmaf(-ax, p * __builtin_amdgcn_exp2f(x * x * -0.72134752f), fmaxf(x, 0.f));
+  return fmaf(-fminf(ax, 1e30f), p * __builtin_amdgcn_exp2f(x * x * -0.72134752f), fmaxf(x, 0.f));
 }
 
 __device__ __forceinline__ uint32_t umax8(const float (&v)[8]) {
@@ -574,9 +575,14 @@ extern "C" int dph_quant_rows_i8(const void* x, int x_f32, int64_t rows, int64_t
                : quant_rows<bf16_t>(x, rows, K, ldx, q, ldq, scale, stream);
 }
 
-// whether x (given, not its integers) goes through the kernel of up to 16 rows, which needs no q
+// whether x (given, not its integers) goes through the kernel of up to 16 rows, which needs no q.  All its workgroups read
+// x while some have written their part of out: where these lie over each other x is quantised first
 static bool small_i8(const DphLinearI8Args& a) {
-  return a.x && a.M <= SMALL_M && a.M * small_ld(a.K) <= SMALL_LDS && a.N > 0;
+  if (!a.x || a.M > SMALL_M || a.M * small_ld(a.K) > SMALL_LDS || a.N <= 0) return false;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.x), o = reinterpret_cast<uintptr_t>(a.out);
+  const int64_t nx = ((a.M - 1) * a.ldx + a.K) * (a.x_f32 ? 4 : 2),
+                no = ((a.M - 1) * a.ldo + a.N) * (a.out_dtype == DPH_OUT_F32 ? 4 : 2);
+  return !o || x + nx <= o || o + no <= x;
 }
 
 extern "C" int64_t dph_linear_i8_workspace(int64_t M, int64_t N, int64_t K) {
@@ -604,6 +610,16 @@ extern "C" int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream) {
     DPH_REQUIRE(a.ldq >= a.K && a.ldq % 16 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0,
                 "dph_linear_i8: rows of q start 16 bytes apart or a multiple of it");
   }
+  auto tiles = [&](int b) { return cdiv(a.M, b) * cdiv(a.N, b); };
+  if (a.N > 0) {
+    DPH_REQUIRE(a.w && a.w_scale && a.out, "dph_linear_i8: null operand");
+    DPH_REQUIRE(a.ldw >= a.K && a.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0,
+                "dph_linear_i8: rows of w start 16 bytes apart or a multiple of it");
+    DPH_REQUIRE(a.ldo >= a.N || a.M == 1, "dph_linear_i8: rows of out overlap");
+    DPH_REQUIRE((small || a.ldq < (1 << 23)) && a.ldw < (1 << 23),
+                "dph_linear_i8: rows of q and w less than 2^23 bytes apart");
+    DPH_REQUIRE(tiles(256) < (1 << 22), "dph_linear_i8: too many tiles");
+  }
   if (a.x) {
     DPH_REQUIRE(a.ldx >= a.K || a.M == 1, "dph_linear_i8: rows of x overlap");
     if (a.ln_weight) {
@@ -622,12 +638,6 @@ extern "C" int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream) {
     }
   }
   if (a.N == 0) return DPH_OK;
-  DPH_REQUIRE(a.w && a.w_scale && a.out, "dph_linear_i8: null operand");
-  DPH_REQUIRE(a.ldw >= a.K && a.ldw % 16 == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0,
-              "dph_linear_i8: rows of w start 16 bytes apart or a multiple of it");
-  DPH_REQUIRE(a.ldo >= a.N || a.M == 1, "dph_linear_i8: rows of out overlap");
-  DPH_REQUIRE((small || a.ldq < (1 << 23)) && a.ldw < (1 << 23),
-              "dph_linear_i8: rows of q and w less than 2^23 bytes apart");
   const int es = out32 ? 4 : 2, res = a.residual ? (out32 ? 2 : 1) : 0;
   const uintptr_t al = reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.residual) |
                        (uintptr_t)(a.ldo * es) | (uintptr_t)(a.residual ? a.ldr * es : 0);
@@ -645,8 +655,6 @@ extern "C" int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream) {
   }
   // Measured on tiles of 256 / 128 / 64, the product alone: 7984 x 1024 x 4096 62 / 45 / 66 us, 8192 x 8192 x 8192 398 / 518 us
   // / -, 7984 x 2304 x 768 32 / 24 / 36 us, 1497 x 768 x 1533 37 / 16 / 15 us
-  auto tiles = [&](int b) { return cdiv(a.M, b) * cdiv(a.N, b); };
-  DPH_REQUIRE(tiles(256) < (1 << 22), "dph_linear_i8: too many tiles");
   auto go = [&](auto c) {
     using C = decltype(c);
     p.ntn = (int32_t)cdiv(a.N, C::BN);

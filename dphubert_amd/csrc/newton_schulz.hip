@@ -28,10 +28,6 @@
 
 #include <type_traits>
 
-
-#ifndef NSW
-#define NSW 16
-#endif
 namespace dph {
 namespace {
 
@@ -299,7 +295,7 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
     koff = (int64_t)kp * g.part_steps * 64 * ld;
     kbytes = min(g.part_steps * 128, kbytes - kp * g.part_steps * 128);
   }
-  using V = mt::Strip<C::FN, C::FN % 4 == 0 ? NSW : 8>;
+  using V = mt::Strip<C::FN, C::FN % 4 == 0 ? 16 : 8>;
   constexpr int NV = 4 * C::FN;
   f32x4_t acc[C::FM][C::FN];
   const int mw = m0 + wave / C::WC * C::WTM + (lane & 15), nw = n0 + wave % C::WC * C::WTN;

@@ -540,6 +540,31 @@ def _chk_i8(dev, r, name):
     return R, K, ld
 
 
+def _bytes(t):
+    """First byte and the one behind the last of a tensor."""
+    p = t.data_ptr()
+    return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else p
+
+
+def _overlap(a, b):
+    (a0, a1), (b0, b1) = _bytes(a), _bytes(b)
+    return a0 < b1 and b0 < a1
+
+
+def _chk_out(out, x, w, bias, residual):
+    """out is the residual itself, beside it (columns of one buffer), or elsewhere, and over no operand; whether it lies
+    over x, which is then quantised first."""
+    if residual is not None and _overlap(out, residual):
+        (ld, N), d = (out.stride(0), out.shape[1]), (out.data_ptr() - residual.data_ptr()) // out.element_size()
+        if (d or out.stride() != residual.stride()) and \
+                not (ld == residual.stride(0) and N <= d % ld <= ld - N):
+            raise ValueError("out overlaps the residual, but is not it")
+    rows = isinstance(x, I8Rows)
+    if any(t is not None and _overlap(out, t) for t in (w.q, w.scale, bias) + (tuple(x) if rows else ())):
+        raise ValueError("out overlaps an operand")
+    return not rows and _overlap(out, x)
+
+
 _F32_ONLY, _I8_ONLY, _FLOATS = (F32,), (torch.int8,), (BF16, F32)
 
 
@@ -608,11 +633,12 @@ def _linear_i8(x, w, bias, act, residual, out, out_dtype, ln, keep_norm):
         with torch.cuda.device(dev):
             return _linear_i8(x, w, bias, act, residual, out, out_dtype, ln, keep_norm)
     if out is None:
-        out, ldo = torch.empty((M, N), dtype=out_dtype, device=dev), N
+        out, ldo, over = torch.empty((M, N), dtype=out_dtype, device=dev), N, False
     else:
         if tuple(_chk_on(dev, out, "out", (out_dtype,), 2)) != (M, N):
             raise ValueError(f"out: expected {(M, N)}, got {tuple(out.shape)}")
         ldo = _chk_rows(out, M, N, "out")
+        over = _chk_out(out, x, w, bias, residual)
     norm = torch.empty((M, K), dtype=BF16, device=dev) if keep_norm else None
     if not M:
         return out, norm
@@ -621,7 +647,7 @@ def _linear_i8(x, w, bias, act, residual, out, out_dtype, ln, keep_norm):
         qp, sp = x.q.data_ptr(), x.scale.data_ptr()
     else:
         xp, xf, ldq, qp, sp = x.data_ptr(), x.dtype == F32, _i8_ld(K), 0, 0
-        nbytes = _lib.lib().dph_linear_i8_workspace(M, N, K)
+        nbytes = M * (ldq + 4) if over else _lib.lib().dph_linear_i8_workspace(M, N, K)
         if nbytes:
             ws = torch.empty((nbytes,), dtype=torch.int8, device=dev)    # q, then the scales
             qp = ws.data_ptr()
@@ -642,7 +668,7 @@ def linear_i8(x: Union[torch.Tensor, I8Rows], w: I8Rows, bias: Optional[torch.Te
     x [M, K] bf16 / fp32 (quantised here, one scale a token) or the I8Rows of it; w: quant_rows_i8 of the nn.Linear
     weight [N, K]; bias [N] fp32; act ACT_NONE / ACT_GELU; residual [M, N] bf16 / fp32, whose type the output takes
     (without one ``out_dtype``).  Integer sums are exact; scales, bias, activation and residual are applied in fp32.
-    K up to 131072.  x, residual and out may be row-strided; out may be the residual itself."""
+    K up to 131072.  x, residual and out may be row-strided; out may be the residual itself, and lie over x."""
     return _linear_i8(x, w, bias, act, residual, out, out_dtype, None, False)[0]
 
 
@@ -672,7 +698,8 @@ NS_COEFFS = (3.4445, -4.7750, 2.0315)
 class NewtonSchulzPlan:
     """The orthogonalisation of one list of matrices, run as often as their contents change (an optimiser's updates): the
     arguments are checked once, results (``out``, bf16, the matrices' shapes) and workspace are kept.  Runs of one plan
-    are ordered by whoever makes them (one stream, or events): they share both."""
+    are ordered by whoever makes them (one stream, or events): they share both.  A graph that captured a run needs the
+    plan for as long as it is replayed."""
 
     def __init__(self, mats: Sequence[torch.Tensor], *, steps: int = 5, coeffs: Sequence[float] = NS_COEFFS,
                  eps: float = 1e-7):
@@ -700,7 +727,7 @@ class NewtonSchulzPlan:
             # (the stride of a dimension of one element is whatever the view says: it is never used)
             places.setdefault((R, K, t.dtype), []).append(
                 (i, t.data_ptr()) + ((max(s0, K), 1) if by_row else (1, max(s1, R))))
-        self.device, self.mats = dev, mats
+        self.device, self.mats, self._at, self._res = dev, mats, [t.data_ptr() for t in mats], []
         self._arr = (_lib.DphNsMat * len(mats))()
         self._grp = (_lib.DphNsGroup * len(places))()
         self._steps, self._eps, self._coeffs = int(steps), float(eps), (C.c_float * 3)(*coeffs)
@@ -709,6 +736,7 @@ class NewtonSchulzPlan:
             k = 0
             for g, ((R, K, dt), at) in zip(self._grp, places.items()):
                 res = torch.empty(len(at), R, K, dtype=BF16, device=dev)
+                self._res.append(res)
                 g.rows, g.cols, g.count, g.out, g.f32 = R, K, len(at), res.data_ptr(), int(dt == F32)
                 for (i, p, rs, cs), o in zip(at, res.unbind()):
                     self.out[i] = o
@@ -718,9 +746,16 @@ class NewtonSchulzPlan:
             if nbytes < 0:
                 _lib.check(-1, "dph_newton_schulz_workspace")
             self._ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            self._home = _stream()
 
     def run(self) -> List[torch.Tensor]:
+        for i, (t, p) in enumerate(zip(self.mats, self._at)):
+            if t.data_ptr() != p:
+                raise RuntimeError(f"mats[{i}] has moved since the plan was made: make another")
         with _on_device(self.device):
+            if _stream() != self._home and not torch.cuda.is_current_stream_capturing():
+                for t in (self._ws, *self._res):        # (they are not handed out again before this stream is done)
+                    t.record_stream(torch.cuda.current_stream())
             call("dph_newton_schulz", self._arr, self._grp, len(self._grp), self._steps, self._coeffs, self._eps,
                  ptr(self._ws), self._ws.numel(), _stream())
         return self.out

@@ -251,16 +251,16 @@ def f32_cat(*ts: torch.Tensor) -> torch.Tensor:
 
 def i8_image(*ts: torch.Tensor) -> "K.I8Rows":
     """Weights (concatenated along dim 0) as 8-bit integers with one scale an output channel (kernels.quant_rows_i8),
-    cached on the first one like bf16_image."""
+    cached on the first one like bf16_image (which keeps the others alive: another tensor cannot take their identity)."""
     owner = ts[0]
-    key = ("i8", owner.device) + _version_key(ts)
+    key = tuple((t.device, t.data_ptr(), t._version) for t in ts)
     hit = getattr(owner, "_dph_i8", None)
-    if hit is not None and hit[0] == key:
+    if hit is not None and hit[0] == key and len(hit[2]) == len(ts) - 1 and all(a is b for a, b in zip(hit[2], ts[1:])):
         return hit[1]
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("8-bit weights changed inside a HIP graph capture: run the model once before it")
     w = ts[0].detach() if len(ts) == 1 else torch.cat([t.detach() for t in ts])
-    owner._dph_i8 = (key, K.quant_rows_i8(w))
+    owner._dph_i8 = (key, K.quant_rows_i8(w), ts[1:])
     return owner._dph_i8[1]
 
 

@@ -197,23 +197,33 @@ class FusedMuon(FusedAdamW):
             raise ValueError(f"momentum must be in [0, 1), got {momentum}")
         if not 1 <= int(ns_steps) <= 64:
             raise ValueError(f"ns_steps must be 1 to 64, got {ns_steps}")
+        self._momentum = momentum
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_grad_norm=max_grad_norm)
-        for g in self.param_groups:
-            if not g.get("muon", False):
-                continue
+        self.nesterov = bool(nesterov)
+        self._ns = dict(steps=int(ns_steps), eps=float(ns_eps))
+        if ns_coeffs is not None:
+            self._ns["coeffs"] = tuple(ns_coeffs)
+        self._muon_key = self._muon_shapes = None
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        if not g.get("muon", False):
+            return
+        try:
             for p in g["params"]:
                 if p.dim() < 2 or p.numel() == 0:
                     raise ValueError(f"muon group: parameters of two or more dimensions, got {tuple(p.shape)}")
                 if p.dtype != torch.float32 or not p.is_contiguous():
                     raise ValueError("muon group: contiguous fp32 parameters")
-            g["momentum"] = g.get("momentum", momentum)
-            # (the kernels' beta1; also what StepScalars uploads)
-            g["betas"] = (g["momentum"], 0.0)
-        self.nesterov = bool(nesterov)
-        self._ns = dict(steps=int(ns_steps), eps=float(ns_eps))
-        if ns_coeffs is not None:
-            self._ns["coeffs"] = tuple(ns_coeffs)
-        self._muon_key = None
+            g["momentum"] = g.get("momentum", self._momentum)
+            if not 0.0 <= g["momentum"] < 1.0:
+                raise ValueError(f"momentum must be in [0, 1), got {g['momentum']}")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+        # (the kernels' beta1; also what StepScalars uploads)
+        g["betas"] = (g["momentum"], 0.0)
 
     def _is_muon(self, gi):
         return bool(self.param_groups[gi].get("muon", False))
@@ -226,13 +236,13 @@ class FusedMuon(FusedAdamW):
         at = [(i, gi, p) for i, (gi, p) in enumerate(plist) if self._is_muon(gi)]
         key = tuple((p.data_ptr(), p.grad.data_ptr() if p.grad is not None else 0,
                      self.state[p]["momentum_buffer"].data_ptr(), dst.get(id(p), 0), p.numel(), gi) for _, gi, p in at)
-        if key == self._muon_key:
+        shapes = tuple((i, tuple(p.shape), p.device) for i, _, p in at) + (len(plist),)
+        if key == self._muon_key and shapes == self._muon_shapes:
             return
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FusedMuon: parameter/gradient storage changed inside a HIP graph capture")
         from . import kernels as K
-        shapes = tuple((tuple(p.shape), p.device) for _, _, p in at)
-        if at and getattr(self, "_muon_shapes", None) != shapes:
+        if at and shapes != self._muon_shapes:
             dev = at[0][2].device
             pad = lambda n: (n + 3) & ~3  # noqa: E731
             flat = torch.zeros(sum(pad(p.numel()) for _, _, p in at), dtype=torch.float32, device=dev)

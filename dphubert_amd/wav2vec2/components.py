@@ -494,10 +494,15 @@ class EncoderLayer(Module):
         if not next(self.parameters()).is_cuda:
             raise ValueError("quantize_int8 runs on the HIP path only: move the model to the device first")
 
-    def int8_weights(self):
-        """The layer's weights as 8-bit integers (cached per parameter version): ops.i8_image."""
+    def int8_weights(self, again: bool = False):
+        """The layer's weights as 8-bit integers (cached per parameter version): ops.i8_image.  again: whatever is cached
+        (a replayed training step changes weights without their versions)."""
         a, f = self.attention, self.feed_forward
         w = {}
+        if again:
+            for p in self.parameters():
+                if hasattr(p, "_dph_i8"):
+                    del p._dph_i8
         if a is not None:
             w["qkv"] = ops.i8_image(a.q_proj.weight, a.k_proj.weight, a.v_proj.weight)
             w["out"] = ops.i8_image(a.out_proj.weight)

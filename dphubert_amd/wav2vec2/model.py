@@ -143,7 +143,7 @@ class Wav2Vec2Model(Module):
         for layer in layers:
             layer.int8 = bool(enable)
             if enable:
-                layer.int8_weights()
+                layer.int8_weights(again=True)
         return self
 
     def prune(self):

@@ -652,8 +652,8 @@ int dph_quant_rows_i8(const void* x, int x_f32, int64_t rows, int64_t K, int64_t
  * ln_weight / ln_bias [K] its LayerNorm (K up to DPH_I8_LN_MAX) is, from the fp32 values; norm_out then receives these
  * in bf16 (NULL: not).  w rows ldw bytes apart (a multiple of 16), bias may be NULL.  act: DPH_ACT_NONE / _GELU.
  * residual (NULL: none) has out's type.  The sums are 32-bit integers, everything after them fp32.  What stands between
- * K and the end of a row of q or w has no effect (it is read up to the next 16 bytes).  out must not overlap an input
- * other than the residual it replaces element for element. */
+ * K and the end of a row of q or w has no effect (it is read up to the next 16 bytes).  out may replace the residual
+ * element for element, and lie over x where q is given; nothing else that is written may overlap an input. */
 typedef struct DphLinearI8Args {
   int64_t M, N, K;
   const void* x;
@@ -680,7 +680,7 @@ typedef struct DphLinearI8Args {
 } DphLinearI8Args;
 int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream);
 /* bytes that x's integers and scales need (q, rows the next multiple of 16 of K apart, then q_scale); 0: q and q_scale may
- * be NULL (up to 16 rows are quantised where they are multiplied) */
+ * be NULL (up to 16 rows are quantised where they are multiplied), unless out lies over x */
 int64_t dph_linear_i8_workspace(int64_t M, int64_t N, int64_t K);
 
 /* ---- Newton-Schulz orthogonalisation (ABI 25) ---------------------------------------------------------------------

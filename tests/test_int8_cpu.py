@@ -61,6 +61,16 @@ def test_c_quant_refuses(kw):
     assert _lib.lib().dph_quant_rows_i8(d["x"], d["f32"], d["rows"], d["K"], d["ldx"], d["q"], d["ldq"], d["scale"], None) == -1
 
 
+@pytest.mark.parametrize("x,out,small", [(4096, 1 << 16, True), (4096, 4096, False), (4096, 4096 + 254, False),
+                                         (4096, 4096 + 256, True), (4096 + 30, 4096, False), (4096 + 32, 4096, True)])
+def test_c_entry_needs_q_where_out_lies_over_x(x, out, small):
+    """Up to 16 rows need no q (a null w is then what is refused), unless bytes of out are bytes of x: 4 rows of 32 bf16
+    columns are 256 bytes, 4 of 4 are 32."""
+    assert _lib.lib().dph_linear_i8(C.byref(_args(x=x, ldx=32, out=out, q=None, q_scale=None, ldw=8)), None) == -1
+    assert (b"rows of w" in _lib.lib().dph_last_error()) == small
+    assert (b"null operand" in _lib.lib().dph_last_error()) == (not small)
+
+
 def test_workspace():
     """Nothing for up to 16 rows that fit the LDS, else the integers (rows of whole 16 bytes) and the scales."""
     ws = _lib.lib().dph_linear_i8_workspace

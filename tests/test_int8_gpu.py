@@ -172,6 +172,50 @@ def test_linear_strides_out_and_in_place():
     assert (room[:, :5] == 7).all() and (room[:, 5 + N:] == 7).all()
 
 
+@pytest.mark.parametrize("M", [4, 16, 40])
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_linear_out_over_x(M, dt):
+    """The residual stream in place: x, the residual and out are one tensor."""
+    g = gen(16)
+    x = acts(M, 640, dt, g)
+    w = K.quant_rows_i8((torch.randn(640, 640, generator=g) / 25).cuda())
+    q, s = rows64(x)
+    want = linear64(q, s, w, None, K.ACT_NONE, x)
+    alone = K.linear_i8(x, w, residual=x)
+    assert K.linear_i8(x, w, residual=x, out=x) is x
+    assert torch.equal(x, alone)
+    check(x, want, want.abs() + 4)
+    # out over x's columns of one buffer, and between them
+    buf = acts(M, 200, dt, g)
+    w = K.quant_rows_i8(torch.randn(50, 100, generator=g).cuda())
+    want = K.linear_i8(buf[:, :100].clone(), w, out_dtype=dt)
+    keep = buf.clone()
+    for c in (150, 50, 0):
+        K.linear_i8(buf[:, :100], w, out=buf[:, c:c + 50], out_dtype=dt)
+        assert torch.equal(buf[:, c:c + 50], want)
+        buf.copy_(keep)
+    # beside the residual in one buffer; across it is refused
+    want = K.linear_i8(buf[:, :100], w, residual=buf[:, 100:150])
+    K.linear_i8(buf[:, :100], w, residual=buf[:, 100:150], out=buf[:, 150:])
+    assert torch.equal(buf[:, 150:], want) and torch.equal(buf[:, :150], keep[:, :150])
+    for bad in (buf[:, 101:151], buf[:, 51:101], buf.view(-1)[100:100 + 50 * M].view(M, 50)):
+        with pytest.raises(ValueError, match="overlaps"):
+            K.linear_i8(buf[:, :100], w, residual=buf[:, 100:150], out=bad)
+    with pytest.raises(ValueError, match="overlaps"):
+        K.linear_i8(buf[:1, :100], w, out=w.scale.view(1, 50), out_dtype=F32)
+
+
+def test_gelu_of_sums_past_the_range():
+    """Finite operands whose sum is infinite in fp32: GELU(inf) = inf, and GELU(-inf) has the limit 0."""
+    for M in (3, 40):
+        x = torch.full((M, 4096), 3e38, device="cuda")
+        w = K.quant_rows_i8(torch.stack([torch.ones(4096), -torch.ones(4096), torch.zeros(4096)]).cuda())
+        y = K.linear_i8(x, w, act=K.ACT_GELU, out_dtype=F32)
+        assert (y[:, 0] == math.inf).all() and not y[:, 1:].any()
+        x[1, 7] = math.nan
+        assert K.linear_i8(x, w, act=K.ACT_GELU).isnan().all(1).tolist() == [r == 1 for r in range(M)]
+
+
 def test_linear_rows_do_not_touch_each_other():
     g = gen(7)
     x = acts(40, 256, F32, g)

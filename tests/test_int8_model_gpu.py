@@ -90,6 +90,25 @@ def test_weights_are_laid_out_again_when_they_change():
         assert not torch.equal(m.extract_features(w, ln)[0][-1], y)
 
 
+def test_weights_that_changed_unseen_are_laid_out_by_the_next_quantize():
+    """A replayed optimiser step, or new storage, changes weights without their versions."""
+    m = _model("hubert", layers=1).quantize_int8()
+    a, lay = m.encoder.transformer.layers[0].int8_weights(), m.encoder.transformer.layers[0]
+    g = torch.cuda.CUDAGraph()
+    p = lay.feed_forward.output_dense.weight
+    with torch.no_grad(), torch.cuda.graph(g):
+        p.mul_(2.0)
+    m.quantize_int8(False).quantize_int8()
+    g.replay()
+    b = m.quantize_int8(False).quantize_int8().encoder.transformer.layers[0].int8_weights()
+    assert torch.equal(b["down"].scale, 2 * a["down"].scale)
+    p.data = p.data * 3
+    assert torch.equal(lay.int8_weights()["down"].q, K.quant_rows_i8(p.detach()).q)
+    # another key projection (whose identity may be the freed one's)
+    lay.attention.k_proj.weight = torch.nn.Parameter(torch.zeros_like(lay.attention.k_proj.weight))
+    assert not lay.int8_weights()["qkv"].q[768:1536].any()
+
+
 def test_forward_only():
     m = _model("hubert", layers=1).quantize_int8()
     w, ln = _wave()

@@ -32,6 +32,17 @@ def test_groups_keep_their_settings():
     assert o.param_groups[0]["momentum"] == 0.9
 
 
+def test_groups_added_later_are_checked_too():
+    o = FusedMuon([{"params": [_p(3, 4)], "muon": True}], momentum=0.9)
+    o.add_param_group({"params": [_p(5, 4)], "muon": True})
+    o.add_param_group({"params": [_p(5)]})
+    assert o.param_groups[1]["momentum"] == 0.9 and o.param_groups[1]["betas"] == (0.9, 0.0) and not o._is_muon(2)
+    for bad in ({"params": [_p(5)], "muon": True}, {"params": [_p(5, 2)], "muon": True, "momentum": 1.0}):
+        with pytest.raises(ValueError):
+            o.add_param_group(bad)
+    assert len(o.param_groups) == 3
+
+
 def _module(**kw):
     from dphubert_amd.synthetic import HUBERT_BASE_CONFIG
     from dphubert_amd.trainer import build_distill_module

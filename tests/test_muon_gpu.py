@@ -78,6 +78,24 @@ def test_parameter_without_gradient_is_left_alone():
     assert torch.equal(a, moved) and not torch.equal(b, before)
 
 
+def test_group_added_after_a_step_moves():
+    g = gen(12)
+    a, b, c = params([(40, 30), (7,), (20, 50)], g)
+    opt = FusedMuon([{"params": [a], "lr": 1e-2, "muon": True}])
+    a.grad = torch.randn_like(a)
+    opt.step()
+    opt.add_param_group({"params": [b], "lr": 1e-2, "weight_decay": 0.0})
+    for add in (None, {"params": [c], "lr": 1e-2, "muon": True}):
+        if add:
+            opt.add_param_group(add)
+        ps = [a, b, c] if add else [a, b]
+        old = [p.detach().clone() for p in ps]
+        for p in ps:
+            p.grad = torch.randn_like(p)
+        opt.step()
+        assert all((p != q).any() for p, q in zip(ps, old))
+
+
 def test_writes_bf16_images():
     g = gen(3)
     ps = params([(96, 64), (96, 64), (96, 64), (50, 3)], g)

@@ -202,6 +202,25 @@ def test_graph_replays_on_other_inputs_and_streams():
         assert torch.equal(x, y)
 
 
+def test_plan_on_another_stream_and_after_a_move():
+    g = gen(13)
+    mats = [noise(100, 70, g), noise(130, 300, g)]
+    plan = K.NewtonSchulzPlan(mats)
+    want = [t.clone() for t in plan.run()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = plan.run()
+    del plan                                       # (its workspace is still being read)
+    junk = [torch.full((1 << 20,), 7.0, device="cuda") for _ in range(8)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and len(junk) == 8
+    plan = K.NewtonSchulzPlan(mats)
+    mats[1].data = mats[1].clone()
+    with pytest.raises(RuntimeError, match="moved"):
+        plan.run()
+
+
 def test_refuses_what_it_does_not_take():
     x = torch.randn(8, 9, device="cuda")
     for bad in ([x.half()], [x[0]], [x.double()], [x[:0]], [x.cpu()], [x, x.cpu()], [x[:, ::2][::2]], [x.expand(8, 9)[:1].expand(8, 9)]):
