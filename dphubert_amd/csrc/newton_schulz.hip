@@ -44,7 +44,11 @@ constexpr int NS_DEEP = 256, NS_LONG = 1024;
 
 __device__ __forceinline__ f16_t f2h(float v) { return __builtin_bit_cast(f16_t, (_Float16)v); }
 __device__ __forceinline__ float h2f(f16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
-__device__ __forceinline__ uint32_t pack2h(float a, float b) { return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16); }
+__device__ __forceinline__ uint32_t pack2h(float a, float b) {
+  typedef __attribute__((ext_vector_type(2))) float f2;
+  typedef __attribute__((ext_vector_type(2))) _Float16 h2;
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), h2));
+}
 __device__ __forceinline__ void unpack4h(uint2 r, float* v) {
   v[0] = h2f((f16_t)(r.x & 0xffff)); v[1] = h2f((f16_t)(r.x >> 16));
   v[2] = h2f((f16_t)(r.y & 0xffff)); v[3] = h2f((f16_t)(r.y >> 16));
@@ -63,16 +67,18 @@ __device__ __forceinline__ uint32_t low4q(const float* v, uint2 h) {
   float q[4];
   unpack4h(h, q);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) q[r] = fminf(fmaxf((v[r] - q[r]) * LO_UP, -448.f), 448.f);
+  for (int r = 0; r < 4; ++r) q[r] = fminf(fmaxf(fmaf(q[r], -LO_UP, v[r] * LO_UP), -448.f), 448.f);
   const int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
 }
-__device__ __forceinline__ void add_low4q(float* v, uint32_t w) {
+// v = (v + what w holds) scale
+__device__ __forceinline__ void add_low4q(float* v, uint32_t w, float scale) {
   const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-  v[0] += a[0] * (1.f / LO_UP);
-  v[1] += a[1] * (1.f / LO_UP);
-  v[2] += b[0] * (1.f / LO_UP);
-  v[3] += b[1] * (1.f / LO_UP);
+  const float l = scale * (1.f / LO_UP);
+  v[0] = fmaf(v[0], scale, a[0] * l);
+  v[1] = fmaf(v[1], scale, a[1] * l);
+  v[2] = fmaf(v[2], scale, b[0] * l);
+  v[3] = fmaf(v[3], scale, b[1] * l);
 }
 
 // Matrices of one shape: cnt of them, Y n x m (m <= n) in rows padded with zeros to multiples of 64 (np, mp)
@@ -105,7 +111,7 @@ struct Step {
   float d, fe, fq, mu, fd; // E = A - d I;  F = fe E + fq E^2 + fd I;  Y <- mu Y + Y F
   int32_t reverse;         // tiles from the last to the first
   int32_t cur;             // which y is read
-  int32_t lo_in, lo_out;   // Y's 8 bits more are read, written
+  int32_t lo_out;          // Y's 8 bits more are written (they are read where mu is not 0)
 };
 struct PackGroup {
   int32_t m, n, mp, np, in_f32;
@@ -300,43 +306,51 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
   f32x4_t acc[C::FM][C::FN];
   const int mw = m0 + wave / C::WC * C::WTM + (lane & 15), nw = n0 + wave % C::WC * C::WTN;
   const int M = SYM ? g.mp : g.np, N = g.mp;      // (what lies past m and n is zero, and stays zero)
-  // the sums start from 0, or from mu Y, whose rows are about to be read as an operand anyway
+  // the sums start from 0, or from mu Y, whose rows are about to be read as an operand anyway.  All its reads are asked for
+  // before the first is used, and rows past the end read the last one instead of none (a read inside a branch is waited
+  // for there: 16 latencies one after the other, 280 against 200 us for the update of 24 matrices of 4096 x 1024)
   auto init = [&]() {
     if (SYM || st.mu == 0.f) {
       mt::clear<T, C>(acc);
     } else {
       const float mu = st.mu * NS_E;
+      using Low = std::conditional_t<SPLIT, uint4, uint2>;
+      uint4 h[C::FM][NV / 8];
+      Low l[C::FM][NV / 8];
 #pragma unroll
       for (int i = 0; i < C::FM; ++i) {
-        const int m = mw + 16 * i;
+        const int64_t row = yoff / 2 + (int64_t)min(mw + 16 * i, M - 1) * N;
+#pragma unroll
+        for (int c = 0; c < NV; c += 8) {
+          const int64_t o = row + min(nw + V::col(c / V::W, lane), N - V::W) + c % V::W;
+          h[i][c / 8] = *reinterpret_cast<const uint4*>(g.y[st.cur] + 2 * o);
+          if constexpr (SPLIT) l[i][c / 8] = *reinterpret_cast<const uint4*>(g.yl[st.cur] + 2 * o);
+          else l[i][c / 8] = *reinterpret_cast<const uint2*>(g.lo + o);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < C::FM; ++i) {
         float x[NV];
 #pragma unroll
-        for (int q = 0; q < V::NG; ++q) {
-          const int n = nw + V::col(q, lane);
-          const bool in = m < M && n < N;
-          const int64_t o = yoff / 2 + (int64_t)m * N + n;
+        for (int c = 0; c < NV; c += 8) {
+          const uint4 hi = h[i][c / 8];
+          const Low lo = l[i][c / 8];
+          unpack4h(make_uint2(hi.x, hi.y), x + c);
+          unpack4h(make_uint2(hi.z, hi.w), x + c + 4);
+          if constexpr (SPLIT) {
+            float f[8];
+            unpack4h(make_uint2(lo.x, lo.y), f);
+            unpack4h(make_uint2(lo.z, lo.w), f + 4);
 #pragma unroll
-          for (int c = 0; c < V::W; c += 8) {
-            const uint4 h = in ? *reinterpret_cast<const uint4*>(g.y[st.cur] + 2 * (o + c)) : make_uint4(0, 0, 0, 0);
-            unpack4h(make_uint2(h.x, h.y), x + V::W * q + c);
-            unpack4h(make_uint2(h.z, h.w), x + V::W * q + c + 4);
-            if (SPLIT) {
-              const uint4 l = in ? *reinterpret_cast<const uint4*>(g.yl[st.cur] + 2 * (o + c)) : make_uint4(0, 0, 0, 0);
-              float lo[8];
-              unpack4h(make_uint2(l.x, l.y), lo);
-              unpack4h(make_uint2(l.z, l.w), lo + 4);
-#pragma unroll
-              for (int r = 0; r < 8; ++r) x[V::W * q + c + r] += lo[r];
-            } else if (st.lo_in) {
-              const uint2 l = in ? *reinterpret_cast<const uint2*>(g.lo + o + c) : make_uint2(0, 0);
-              add_low4q(x + V::W * q + c, l.x);
-              add_low4q(x + V::W * q + c + 4, l.y);
-            }
+            for (int r = 0; r < 8; ++r) x[c + r] = (x[c + r] + f[r]) * mu;
+          } else {
+            add_low4q(x + c, lo.x, mu);
+            add_low4q(x + c + 4, lo.y, mu);
           }
         }
         uint32_t b[NV];
 #pragma unroll
-        for (int r = 0; r < NV; ++r) b[r] = __float_as_uint(x[r] * mu);
+        for (int r = 0; r < NV; ++r) b[r] = __float_as_uint(x[r]);
         V::exchange(b);
 #pragma unroll
         for (int r = 0; r < NV; ++r) acc[i][r >> 2][r & 3] = __uint_as_float(b[r]);
@@ -378,6 +392,19 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
     return;
   }
 
+  // (E, like Y above: all of the tile before the first store)
+  constexpr int NE = KIND == POLY ? NV / 4 : 1;
+  uint2 e_hi[C::FM][NE], e_lo[C::FM][SPLIT ? NE : 1];
+  if constexpr (KIND == POLY) {
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int c = 0; c < NV; c += 4) {
+        const int64_t o = (int64_t)min(mw + 16 * i, M - 1) * N + min(nw + V::col(c / V::W, lane), N - V::W) + c % V::W;
+        e_hi[i][c / 4] = *reinterpret_cast<const uint2*>(g.e + eoff + o * 2);
+        if constexpr (SPLIT) e_lo[i][c / 4] = *reinterpret_cast<const uint2*>(g.el + eoff + o * 2);
+      }
+  }
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
     const int m = mw + 16 * i;
@@ -397,27 +424,26 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
         char* to = (KIND == GRAM ? g.e : g.f) + eoff;
         char* tl = (KIND == GRAM ? g.el : g.fl) + eoff;
         const int64_t o = (int64_t)m * N + n0q;
+        const float diag = m < g.m ? NS_E * (KIND == GRAM ? st.d : st.fd) : 0.f;
         if constexpr (KIND == GRAM) {
           const float sc = NS_E / (g.s * g.s);
 #pragma unroll
-          for (int r = 0; r < V::W; ++r) v[r] = v[r] * sc - (m == n0q + r && m < g.m ? NS_E * st.d : 0.f);
+          for (int r = 0; r < V::W; ++r) v[r] = v[r] * sc - (m == n0q + r ? diag : 0.f);
         } else {
 #pragma unroll
           for (int r = 0; r < V::W; ++r) v[r] *= st.fq / NS_E;
 #pragma unroll
           for (int c = 0; c < V::W; c += 4) {
-            float e[4] = {0.f, 0.f, 0.f, 0.f};
-            if (in) {
-              unpack4h(*reinterpret_cast<const uint2*>(g.e + eoff + (o + c) * 2), e);
-              if constexpr (SPLIT) {
-                float lo[4];
-                unpack4h(*reinterpret_cast<const uint2*>(g.el + eoff + (o + c) * 2), lo);
+            float e[4];
+            unpack4h(e_hi[i][(V::W * q + c) / 4], e);
+            if constexpr (SPLIT) {
+              float lo[4];
+              unpack4h(e_lo[i][(V::W * q + c) / 4], lo);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) e[r] += lo[r];
-              }
+              for (int r = 0; r < 4; ++r) e[r] += lo[r];
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[c + r] += st.fe * e[r] + (m == n0q + c + r && m < g.m ? NS_E * st.fd : 0.f);
+            for (int r = 0; r < 4; ++r) v[c + r] += st.fe * e[r] + (m == n0q + c + r ? diag : 0.f);
           }
         }
 #pragma unroll
@@ -662,7 +688,6 @@ int run_groups(const DphNsMat* mats, const DphNsGroup* groups, int ng, int steps
     st.mu = late ? 0.f : mu;
     st.fd = late ? mu : 0.f;
     st.cur = i & 1;
-    st.lo_in = !late;
     st.lo_out = !(steps - i - 1 <= 2 && steps >= 4);
     DPH_TRY(launch_product<GRAM>(gs, st, stream));
     st.reverse ^= 1;
