@@ -19,9 +19,8 @@ constexpr float SCALE_MIN = 1.17549435e-38f;   // 2^-126: the scale of a row of 
 __device__ __forceinline__ int quant1(float x, float inv, float s) {
   float t = rintf(x * inv);
   const float d = fmaf(-t, s, x), a = fabsf(d), h = 0.5f * s;
-  const bool odd = ((int)t & 1) != 0;
-  if (a > h || (a == h && odd)) t += d > 0.f ? 1.f : -1.f;
-  return (int)t;
+  const int i = (int)t, off = (int)(a > h) | ((int)(a == h) & i);
+  return i + (off & 1 ? (d > 0.f ? 1 : -1) : 0);
 }
 
 // 16 bytes at any alignment of the element (one load: the hardware takes it)
@@ -231,31 +230,26 @@ struct LinearI8 {
   int32_t vec;   // rows of res and out are 16-byte aligned
 };
 
-// W consecutive columns of the residual's row m from n on, as they are in memory (zeros past N).  RES: 0 none, 1 bf16, 2 fp32
+// W consecutive columns of the residual's row m from n on, as they are in memory: VEC in one read, else one by one with
+// zeros past N.  RES: 0 none, 1 bf16, 2 fp32
 template <int W, int RES>
 struct Resid {
   uint32_t w[RES == 2 ? W : W / 2];
+  template <bool VEC>
   __device__ __forceinline__ void load(const LinearI8& a, int64_t m, int n) {
     const int64_t o = m * a.ldr + n;
-    if constexpr (RES == 1) {
+    if constexpr (VEC) {
+      const uint4 r = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(a.res) + o * (RES == 2 ? 4 : 2));
+      w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+    } else if constexpr (RES == 1) {
       const bf16_t* p = reinterpret_cast<const bf16_t*>(a.res) + o;
-      if (a.vec && n + W <= a.N) {
-        const uint4 r = *reinterpret_cast<const uint4*>(p);
-        w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
-      } else {
 #pragma unroll
-        for (int c = 0; c < W; c += 2)
-          w[c / 2] = (n + c < a.N ? (uint32_t)p[c] : 0u) | (n + c + 1 < a.N ? (uint32_t)p[c + 1] << 16 : 0u);
-      }
+      for (int c = 0; c < W; c += 2)
+        w[c / 2] = (n + c < a.N ? (uint32_t)p[c] : 0u) | (n + c + 1 < a.N ? (uint32_t)p[c + 1] << 16 : 0u);
     } else if constexpr (RES == 2) {
       const float* p = reinterpret_cast<const float*>(a.res) + o;
-      if (a.vec && n + W <= a.N) {
-        const uint4 r = *reinterpret_cast<const uint4*>(p);
-        w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
-      } else {
 #pragma unroll
-        for (int c = 0; c < W; ++c) w[c] = n + c < a.N ? __float_as_uint(p[c]) : 0u;
-      }
+      for (int c = 0; c < W; ++c) w[c] = n + c < a.N ? __float_as_uint(p[c]) : 0u;
     }
   }
   __device__ __forceinline__ float get(int c) const {
@@ -266,7 +260,7 @@ struct Resid {
 };
 
 // The row's W sums v, finished and stored (the output has the residual's type; without one it is bf16, or fp32 with OUT32)
-template <int W, bool GELU, int RES, bool OUT32>
+template <int W, bool GELU, int RES, bool OUT32, bool VEC>
 __device__ __forceinline__ void finish(const LinearI8& a, int64_t m, int n, float xs, const float* ws, const float* bias,
                                        const Resid<W, RES>& t, float* v) {
   static_assert(W == (OUT32 ? 4 : 8), "16 bytes");
@@ -277,10 +271,9 @@ __device__ __forceinline__ void finish(const LinearI8& a, int64_t m, int n, floa
     if (GELU) v[c] = gelu_i8(v[c]);
     if constexpr (RES != 0) v[c] += t.get(c);
   }
-  const bool vec = a.vec && n + W <= a.N;
   if constexpr (OUT32) {
     float* p = reinterpret_cast<float*>(a.out) + o;
-    if (vec) {
+    if constexpr (VEC) {
       *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
 #pragma unroll
@@ -289,7 +282,7 @@ __device__ __forceinline__ void finish(const LinearI8& a, int64_t m, int n, floa
     }
   } else {
     bf16_t* p = reinterpret_cast<bf16_t*>(a.out) + o;
-    if (vec) {
+    if constexpr (VEC) {
       *reinterpret_cast<uint4*>(p) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
     } else {
 #pragma unroll
@@ -329,32 +322,38 @@ template <class C, bool GELU, int RES, bool OUT32>
 __device__ __forceinline__ void store_tile(const LinearI8& a, const mt::i32x4_t (&acc)[C::FM][C::FN],
                                            const Scales<C>& sc, int m0, int n0, int wave, int lane) {
   using V = mt::Strip<C::FN, OUT32 ? 4 : 8>;
-  const int mt0 = wave / C::WC * C::WTM + (lane & 15), nt0 = wave % C::WC * C::WTN;
+  const int wn = wave % C::WC * C::WTN, mt0 = wave / C::WC * C::WTM + (lane & 15);
+  auto rows = [&](auto vec) {
+    constexpr bool VEC = decltype(vec)::value;
 #pragma unroll
-  for (int i = 0; i < C::FM; ++i) {
-    const int mt = mt0 + 16 * i, m = m0 + mt;
-    // (a fragment row's residual just before its stores: with two or more rows asked for ahead, reads and writes come in
-    // bursts, 107 against 99 us at 7984 x 4096 x 1024 in fp32)
-    Resid<V::W, RES> t[V::NG];
+    for (int i = 0; i < C::FM; ++i) {
+      const int mt = mt0 + 16 * i, m = m0 + mt;
+      // (a fragment row's residual when the row before is stored: asked for two, four or eight rows early, reads and writes
+      // come in bursts, 86, 89 and 98 us against 86 at 7984 x 4096 x 1024 in fp32)
+      Resid<V::W, RES> t[V::NG];
+      if constexpr (RES != 0) {
 #pragma unroll
-    for (int q = 0; q < V::NG; ++q) {
-      const int n = n0 + nt0 + V::col(q, lane);
-      if (RES != 0 && m < a.M && n < a.N) t[q].load(a, m, n);
+        for (int q = 0; q < V::NG; ++q) t[q].template load<VEC>(a, min(m, a.M - 1), n0 + wn + V::col(q, lane));
+      }
+      uint32_t b[4 * C::FN];
+#pragma unroll
+      for (int r = 0; r < 4 * C::FN; ++r) b[r] = (uint32_t)acc[i][r >> 2][r & 3];
+      V::exchange(b);
+      const float xs = sc.xs[mt];
+#pragma unroll
+      for (int q = 0; q < V::NG; ++q) {
+        const int nt = wn + V::col(q, lane);
+        float v[V::W];
+#pragma unroll
+        for (int r = 0; r < V::W; ++r) v[r] = (float)(int32_t)b[V::W * q + r];
+        if (m < a.M) finish<V::W, GELU, RES, OUT32, VEC>(a, m, n0 + nt, xs, sc.ws + nt, sc.bias + nt, t[q], v);
+      }
     }
-    uint32_t b[4 * C::FN];
-#pragma unroll
-    for (int r = 0; r < 4 * C::FN; ++r) b[r] = (uint32_t)acc[i][r >> 2][r & 3];
-    V::exchange(b);
-    const float xs = sc.xs[mt];
-#pragma unroll
-    for (int q = 0; q < V::NG; ++q) {
-      const int nt = nt0 + V::col(q, lane), n = n0 + nt;
-      float v[V::W];
-#pragma unroll
-      for (int r = 0; r < V::W; ++r) v[r] = (float)(int32_t)b[V::W * q + r];
-      if (m < a.M && n < a.N) finish<V::W, GELU, RES, OUT32>(a, m, n, xs, sc.ws + nt, sc.bias + nt, t[q], v);
-    }
-  }
+  };
+  // a wave's strip of whole vectors has no branch but the one on the row (a read inside a branch is waited for there, alone:
+  // 109 us instead of 86)
+  if (a.vec && n0 + wn + C::WTN <= a.N) rows(std::true_type{});
+  else rows(std::false_type{});
 }
 
 template <class C, bool GELU, int RES, bool OUT32>
