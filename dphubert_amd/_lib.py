@@ -87,6 +87,7 @@ class DphMuonSlot(C.Structure):
 
 I8_K_MAX = 131072
 I8_LN_MAX = 2048
+NS_COEFF_MAX = 256.0
 
 S = vp  # hipStream_t
 

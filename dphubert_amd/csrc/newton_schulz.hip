@@ -85,7 +85,7 @@ __device__ __forceinline__ void add_low4q(float* v, uint32_t w, float scale) {
 struct Group {
   int32_t m, n, mp, np, cnt, wide;    // wide: the caller's matrices are m x n
   float s;                            // Y is held times s
-  int32_t in_f32;
+  int32_t vec;                        // rows of out are 16-byte aligned
   char *y[2], *lo, *yl[2];            // [cnt][np][mp]: fp16 x 2, then e4m3, or (split) two fp16 halves more
   char *e, *f, *el, *fl;              // [cnt][mp][mp]; the lower halves (split) or null
   double* part;                       // [cnt][NS_PARTS]
@@ -242,14 +242,14 @@ enum { GRAM, POLY, UPDATE, LAST };
 // 4 x 4 transpose inside a quad of lanes: lane q of the quad has element (row q, column r) as the r-th of 4 16-bit
 // numbers and leaves with (row r, column q)
 __device__ __forceinline__ uint2 quad_transpose(uint2 x, int lane) {
-  const bool o1 = lane & 1, o2 = lane & 2;
+  // (byte permutes with a lane's own selector: written as conditions, they are compiled to branches)
+  const uint32_t s1 = lane & 1 ? 0x03020706u : 0x05040100u, s2 = lane & 2 ? 0x07060504u : 0x03020100u;
   const uint32_t y0 = (uint32_t)__builtin_amdgcn_mov_dpp((int)x.x, 0xb1, 0xf, 0xf, true);   // lane ^ 1
   const uint32_t y1 = (uint32_t)__builtin_amdgcn_mov_dpp((int)x.y, 0xb1, 0xf, 0xf, true);
-  const uint32_t a0 = o1 ? (y0 >> 16) | (x.x & 0xffff0000u) : (x.x & 0xffffu) | (y0 << 16);
-  const uint32_t a1 = o1 ? (y1 >> 16) | (x.y & 0xffff0000u) : (x.y & 0xffffu) | (y1 << 16);
+  const uint32_t a0 = __builtin_amdgcn_perm(y0, x.x, s1), a1 = __builtin_amdgcn_perm(y1, x.y, s1);
   const uint32_t b0 = (uint32_t)__builtin_amdgcn_mov_dpp((int)a0, 0x4e, 0xf, 0xf, true);    // lane ^ 2
   const uint32_t b1 = (uint32_t)__builtin_amdgcn_mov_dpp((int)a1, 0x4e, 0xf, 0xf, true);
-  return o2 ? make_uint2(b1, a1) : make_uint2(a0, b0);
+  return make_uint2(__builtin_amdgcn_perm(b1, a0, s2), __builtin_amdgcn_perm(a1, b0, s2));
 }
 
 // FINISH: the Gram matrix's parts are added, and no product is made
@@ -292,6 +292,14 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
     ti = t / tm;         // (consecutive tiles share rows of Y)
     tj = t % tm;
   }
+  // the last product in the caller's order: a wide matrix is F Y^T (the operands change places), so that a lane has columns
+  // of it next to each other
+  const bool flip = KIND == LAST && g.wide;
+  if (flip) {
+    static_assert(KIND != LAST || C::BM == C::BN, "square tiles");
+    const int x = ti;
+    ti = tj, tj = x;
+  }
   const int m0 = ti * C::BM, n0 = tj * C::BN;
   const int64_t yoff = (int64_t)z * g.np * g.mp * 2, eoff = (int64_t)z * g.mp * g.mp * 2;
   int kbytes = (KIND == GRAM ? g.np : g.mp) * 2;
@@ -305,12 +313,14 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
   constexpr int NV = 4 * C::FN;
   f32x4_t acc[C::FM][C::FN];
   const int mw = m0 + wave / C::WC * C::WTM + (lane & 15), nw = n0 + wave % C::WC * C::WTN;
-  const int M = SYM ? g.mp : g.np, N = g.mp;      // (what lies past m and n is zero, and stays zero)
+  [[maybe_unused]] const int M = SYM ? g.mp : g.np, N = g.mp;      // (what lies past m and n is zero, and stays zero)
   // the sums start from 0, or from mu Y, whose rows are about to be read as an operand anyway.  All its reads are asked for
   // before the first is used, and rows past the end read the last one instead of none (a read inside a branch is waited
   // for there: 16 latencies one after the other, 280 against 200 us for the update of 24 matrices of 4096 x 1024)
   auto init = [&]() {
-    if (SYM || st.mu == 0.f) {
+    if constexpr (KIND != UPDATE) {
+      mt::clear<T, C>(acc);
+    } else if (st.mu == 0.f) {
       mt::clear<T, C>(acc);
     } else {
       const float mu = st.mu * NS_E;
@@ -379,6 +389,10 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
     } else {
       A = mt::Rows{(la ? g.yl[st.cur] : g.y[st.cur]) + yoff, ld, g.np};
       B = mt::Rows{(lb ? g.fl : g.f) + eoff, ld, g.mp};
+      if (flip) {
+        const mt::Rows x = A;
+        A = B, B = x;
+      }
     }
     mt::product_of<T, C>(A, B, kbytes, m0, n0, acc, smem, wave, lane, [&]() {
       if (!SPLIT || part == 0) init();
@@ -392,6 +406,10 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
     return;
   }
 
+  // (the lane anew: what init() worked out from it is not kept through the product, where every register is taken)
+  int le = lane;
+  asm volatile("" : "+v"(le));
+  const int me = m0 + wave / C::WC * C::WTM + (le & 15);
   // (E, like Y above: all of the tile before the first store)
   constexpr int NE = KIND == POLY ? NV / 4 : 1;
   uint2 e_hi[C::FM][NE], e_lo[C::FM][SPLIT ? NE : 1];
@@ -400,35 +418,35 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
     for (int i = 0; i < C::FM; ++i)
 #pragma unroll
       for (int c = 0; c < NV; c += 4) {
-        const int64_t o = (int64_t)min(mw + 16 * i, M - 1) * N + min(nw + V::col(c / V::W, lane), N - V::W) + c % V::W;
+        const int64_t o = (int64_t)min(me + 16 * i, M - 1) * N + min(nw + V::col(c / V::W, le), N - V::W) + c % V::W;
         e_hi[i][c / 4] = *reinterpret_cast<const uint2*>(g.e + eoff + o * 2);
         if constexpr (SPLIT) e_lo[i][c / 4] = *reinterpret_cast<const uint2*>(g.el + eoff + o * 2);
       }
   }
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
-    const int m = mw + 16 * i;
+    const int m = me + 16 * i;
     uint32_t b[NV];
 #pragma unroll
     for (int r = 0; r < NV; ++r) b[r] = __float_as_uint(acc[i][r >> 2][r & 3]);
     V::exchange(b);
 #pragma unroll
     for (int q = 0; q < V::NG; ++q) {
-      const int n0q = nw + V::col(q, lane);
-      const bool in = m < M && n0q < N;
+      const int n0q = nw + V::col(q, le);
+      [[maybe_unused]] const bool in = m < M && n0q < N;
       float v[V::W];
       uint2 h[V::W / 4];
+      [[maybe_unused]] uint2 l[V::W / 4];
 #pragma unroll
       for (int r = 0; r < V::W; ++r) v[r] = __uint_as_float(b[V::W * q + r]);
       if constexpr (SYM) {
         char* to = (KIND == GRAM ? g.e : g.f) + eoff;
         char* tl = (KIND == GRAM ? g.el : g.fl) + eoff;
         const int64_t o = (int64_t)m * N + n0q;
-        const float diag = m < g.m ? NS_E * (KIND == GRAM ? st.d : st.fd) : 0.f;
         if constexpr (KIND == GRAM) {
           const float sc = NS_E / (g.s * g.s);
 #pragma unroll
-          for (int r = 0; r < V::W; ++r) v[r] = v[r] * sc - (m == n0q + r ? diag : 0.f);
+          for (int r = 0; r < V::W; ++r) v[r] *= sc;
         } else {
 #pragma unroll
           for (int r = 0; r < V::W; ++r) v[r] *= st.fq / NS_E;
@@ -443,69 +461,79 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
               for (int r = 0; r < 4; ++r) e[r] += lo[r];
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[c + r] += st.fe * e[r] + (m == n0q + c + r ? diag : 0.f);
+            for (int r = 0; r < 4; ++r) v[c + r] += st.fe * e[r];
           }
+        }
+        if (ti == tj) {
+          const uint32_t diag = __float_as_uint(m < g.m ? NS_E * (KIND == GRAM ? -st.d : st.fd) : 0.f);
+#pragma unroll
+          for (int r = 0; r < V::W; ++r) v[r] += __uint_as_float(diag & -(uint32_t)(m == n0q + r));
         }
 #pragma unroll
         for (int c = 0; c < V::W / 4; ++c) {
           h[c] = make_uint2(pack2h(v[4 * c], v[4 * c + 1]), pack2h(v[4 * c + 2], v[4 * c + 3]));
-          const uint2 ht = quad_transpose(h[c], lane);
-          const int64_t ot = (int64_t)(n0q + 4 * c + (lane & 3)) * M + (m & ~3);
-          if (ti != tj && in) *reinterpret_cast<uint2*>(to + ot * 2) = ht;
-          if constexpr (SPLIT) {
-            const uint2 l = low4h(v + 4 * c, h[c]), lt = quad_transpose(l, lane);
-            if (in) *reinterpret_cast<uint2*>(tl + (o + 4 * c) * 2) = l;
-            if (ti != tj && in) *reinterpret_cast<uint2*>(tl + ot * 2) = lt;
+          if constexpr (SPLIT) l[c] = low4h(v + 4 * c, h[c]);
+        }
+        // a tile below the diagonal is stored a second time, transposed
+        uint2 ht[V::W / 4], lt[V::W / 4];
+        const int64_t ot = (int64_t)(n0q + (le & 3)) * M + (m & ~3);
+        if (ti != tj) {
+#pragma unroll
+          for (int c = 0; c < V::W / 4; ++c) {
+            ht[c] = quad_transpose(h[c], le);
+            if constexpr (SPLIT) lt[c] = quad_transpose(l[c], le);
           }
         }
         if (in) {
 #pragma unroll
-          for (int c = 0; c < V::W / 4; c += 2)
+          for (int c = 0; c < V::W / 4; c += 2) {
             *reinterpret_cast<uint4*>(to + (o + 4 * c) * 2) = make_uint4(h[c].x, h[c].y, h[c + 1].x, h[c + 1].y);
+            if constexpr (SPLIT)
+              *reinterpret_cast<uint4*>(tl + (o + 4 * c) * 2) = make_uint4(l[c].x, l[c].y, l[c + 1].x, l[c + 1].y);
+          }
+          if (ti != tj) {
+#pragma unroll
+            for (int c = 0; c < V::W / 4; ++c) {
+              *reinterpret_cast<uint2*>(to + (ot + 4 * c * (int64_t)M) * 2) = ht[c];
+              if constexpr (SPLIT) *reinterpret_cast<uint2*>(tl + (ot + 4 * c * (int64_t)M) * 2) = lt[c];
+            }
+          }
         }
       } else if constexpr (KIND == UPDATE) {
         if (in) {
           const int64_t o = yoff / 2 + (int64_t)m * N + n0q;
-          uint32_t l[V::W / 4];
 #pragma unroll
           for (int r = 0; r < V::W; ++r) v[r] *= 1.f / NS_E;
 #pragma unroll
           for (int c = 0; c < V::W / 4; ++c) {
             h[c] = make_uint2(pack2h(v[4 * c], v[4 * c + 1]), pack2h(v[4 * c + 2], v[4 * c + 3]));
             if constexpr (SPLIT) *reinterpret_cast<uint2*>(g.yl[st.cur ^ 1] + 2 * (o + 4 * c)) = low4h(v + 4 * c, h[c]);
-            else if (st.lo_out) l[c] = low4q(v + 4 * c, h[c]);
+            else if (st.lo_out) l[c].x = low4q(v + 4 * c, h[c]);
           }
 #pragma unroll
           for (int c = 0; c < V::W / 4; c += 2)
             *reinterpret_cast<uint4*>(g.y[st.cur ^ 1] + 2 * (o + 4 * c)) =
                 make_uint4(h[c].x, h[c].y, h[c + 1].x, h[c + 1].y);
           if (!SPLIT && st.lo_out) {
-            if constexpr (V::W == 16) *reinterpret_cast<uint4*>(g.lo + o) = make_uint4(l[0], l[1], l[2], l[3]);
-            else *reinterpret_cast<uint2*>(g.lo + o) = make_uint2(l[0], l[1]);
+            if constexpr (V::W == 16) *reinterpret_cast<uint4*>(g.lo + o) = make_uint4(l[0].x, l[1].x, l[2].x, l[3].x);
+            else *reinterpret_cast<uint2*>(g.lo + o) = make_uint2(l[0].x, l[1].x);
           }
         }
       } else {
         const float inv = 1.0f / (g.s * NS_E);
+        const int rows = flip ? g.m : g.n, cols = flip ? g.n : g.m;
+        uint32_t w[V::W / 2];
 #pragma unroll
-        for (int c = 0; c < V::W / 4; ++c) {
-          const int n = n0q + 4 * c;
-          h[c] = make_uint2(pack2bf(v[4 * c] * inv, v[4 * c + 1] * inv), pack2bf(v[4 * c + 2] * inv, v[4 * c + 3] * inv));
-          // the caller's order: rows of m, or of n where the matrix is wide
-          int row = m, col = n, cols = g.m, rows = g.n;
-          if (g.wide) {
-            h[c] = quad_transpose(h[c], lane);
-            row = n + (lane & 3), col = m & ~3, cols = g.n, rows = g.m;
-          }
-          bf16_t* p = g.out + (int64_t)z * g.m * g.n + (int64_t)row * cols + col;
-          if (row < rows) {
-            if (col + 4 <= cols && (cols & 3) == 0) {
-              *reinterpret_cast<uint2*>(p) = h[c];
-            } else {
-              const uint32_t w[2] = {h[c].x, h[c].y};
+        for (int r = 0; r < V::W / 2; ++r) w[r] = pack2bf(v[2 * r] * inv, v[2 * r + 1] * inv);
+        bf16_t* p = g.out + (int64_t)z * rows * cols + (int64_t)m * cols + n0q;
+        if (m < rows) {
+          if (g.vec && nw + C::WTN <= cols) {
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (col + r < cols) p[r] = (bf16_t)(w[r >> 1] >> (16 * (r & 1)));
-            }
+            for (int r = 0; r < V::W / 2; r += 4) *reinterpret_cast<uint4*>(p + 2 * r) = make_uint4(w[r], w[r + 1], w[r + 2], w[r + 3]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < V::W; ++r)
+              if (n0q + r < cols) p[r] = (bf16_t)(w[r >> 1] >> (16 * (r & 1)));
           }
         }
       }
@@ -646,14 +674,14 @@ int run_groups(const DphNsMat* mats, const DphNsGroup* groups, int ng, int steps
     g.mp = (int32_t)up64(g.m);
     g.np = (int32_t)up64(g.n);
     g.cnt = (int32_t)in.count;
-    g.in_f32 = in.f32;
+    g.vec = in.cols % 8 == 0 && reinterpret_cast<uintptr_t>(in.out) % 16 == 0;
     g.out = reinterpret_cast<bf16_t*>(in.out);
     // entries of X0 have the mean square 1 / (m n): s is the power of two next below sqrt(m n) / 4, at most 2^14 so
     // that an entry of 1.5 times s is a finite fp16 number
     g.s = 1.f;
     while (g.s < 16384.f && (double)g.s * g.s * 64.0 <= (double)g.m * g.n) g.s *= 2.f;
     ws += group_bytes(in, ws, &g);
-    pg.g[i] = PackGroup{g.m, g.n, g.mp, g.np, g.in_f32, g.s, g.y[0], g.lo, g.yl[0], g.part};
+    pg.g[i] = PackGroup{g.m, g.n, g.mp, g.np, in.f32, g.s, g.y[0], g.lo, g.yl[0], g.part};
   }
   // both packing passes, NS_MATS matrices at a time
   int gi = 0;
@@ -683,12 +711,14 @@ int run_groups(const DphNsMat* mats, const DphNsGroup* groups, int ng, int steps
     st.fe = c[1] + 2.f * c[2] * st.d;
     st.fq = c[2];
     // near the end mu is below 1 and goes into F's diagonal, whose rounding it does not make worse, and Y is read as an
-    // operand only; before, mu Y is added in as many bits as Y has
+    // operand only; before, mu Y is added in as many bits as Y has.  (In the last step of a short run too: its fp16 rounding
+    // is an eighth of the result's to bf16)
     const float mu = c[0] + c[1] * st.d + c[2] * st.d * st.d;
-    st.mu = late ? 0.f : mu;
-    st.fd = late ? mu : 0.f;
+    const bool diag = late || i + 1 == steps;
+    st.mu = diag ? 0.f : mu;
+    st.fd = diag ? mu : 0.f;
     st.cur = i & 1;
-    st.lo_out = !(steps - i - 1 <= 2 && steps >= 4);
+    st.lo_out = steps - i - 1 > (steps >= 4 ? 2 : 1);
     DPH_TRY(launch_product<GRAM>(gs, st, stream));
     st.reverse ^= 1;
     DPH_TRY(launch_product<POLY>(gs, st, stream));
@@ -710,6 +740,9 @@ extern "C" int dph_newton_schulz(const DphNsMat* mats, const DphNsGroup* groups,
   if (n_groups == 0) return DPH_OK;
   DPH_REQUIRE(mats && coeffs && workspace, "dph_newton_schulz: null pointer");
   DPH_REQUIRE(steps >= 1 && steps <= 64, "dph_newton_schulz: 1 to 64 steps (got %lld)", (long long)steps);
+  for (int i = 0; i < 3; ++i)      // (F's entries times 64 are finite fp16 numbers)
+    DPH_REQUIRE(coeffs[i] >= -DPH_NS_COEFF_MAX && coeffs[i] <= DPH_NS_COEFF_MAX, "dph_newton_schulz: coefficients up to %g",
+                DPH_NS_COEFF_MAX);
   DPH_REQUIRE(workspace_bytes >= dph_newton_schulz_workspace(groups, n_groups) &&
                   reinterpret_cast<uintptr_t>(workspace) % 256 == 0,
               "dph_newton_schulz: workspace of %lld bytes, 256-byte aligned, wanted",

@@ -711,8 +711,8 @@ class NewtonSchulzPlan:
         dev = mats[0].device
         if not 1 <= int(steps) <= 64:
             raise ValueError(f"steps must be 1 to 64, got {steps}")
-        if len(coeffs) != 3:
-            raise ValueError(f"coeffs are (a, b, c), got {coeffs}")
+        if len(coeffs) != 3 or not all(abs(c) <= _lib.NS_COEFF_MAX for c in coeffs):
+            raise ValueError(f"coeffs are (a, b, c), each up to {_lib.NS_COEFF_MAX}, got {coeffs}")
         if not eps >= 0.0:
             raise ValueError(f"eps must not be negative, got {eps}")
         places = {}

@@ -685,11 +685,12 @@ int64_t dph_linear_i8_workspace(int64_t M, int64_t N, int64_t K);
 
 /* ---- Newton-Schulz orthogonalisation (ABI 25) ---------------------------------------------------------------------
  * For every matrix G [rows][cols] of the groups (one shape and type each): X0 = G / (|G|_F + eps) (the smaller side
- * first), `steps` times X <- a X + (b A + c A^2) X with A = X X^T and coeffs = {a, b, c}, the result in bf16 to the
+ * first), `steps` times X <- a X + (b A + c A^2) X with A = X X^T and coeffs = {a, b, c} (up to DPH_NS_COEFF_MAX), the result in bf16 to the
  * group's out [count][rows][cols] (dense, 8-byte aligned).  mats: the groups' matrices one after the other; one of a
  * matrix's strides is 1.  Operands are fp16, sums fp32 (newton_schulz.hip).  The result does not depend on the other
  * matrices of the list.  A zero matrix gives zeros, one with an infinity or a NaN gives NaN throughout. */
 #define DPH_NS_MAX 1048576
+#define DPH_NS_COEFF_MAX 256.0
 typedef struct DphNsMat {
   const void* p;
   int64_t row_stride, col_stride;

@@ -226,6 +226,6 @@ def test_refuses_what_it_does_not_take():
     for bad in ([x.half()], [x[0]], [x.double()], [x[:0]], [x.cpu()], [x, x.cpu()], [x[:, ::2][::2]], [x.expand(8, 9)[:1].expand(8, 9)]):
         with pytest.raises(ValueError):
             K.newton_schulz(bad)
-    for kw in (dict(steps=0), dict(steps=65), dict(coeffs=(1.0, 2.0)), dict(eps=-1.0), dict(eps=math.nan)):
+    for kw in (dict(steps=0), dict(steps=65), dict(coeffs=(1.0, 2.0)), dict(coeffs=(257.0, 0.0, 0.0)), dict(coeffs=(1.0, math.nan, 0.0)), dict(eps=-1.0), dict(eps=math.nan)):
         with pytest.raises(ValueError):
             K.newton_schulz([x], **kw)
