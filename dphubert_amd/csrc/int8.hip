@@ -23,13 +23,6 @@ __device__ __forceinline__ int quant1(float x, float inv, float s) {
   return i + (off & 1 ? (d > 0.f ? 1 : -1) : 0);
 }
 
-// 16 bytes at any alignment of the element (one load: the hardware takes it)
-__device__ __forceinline__ uint4 ld16(const void* p) {
-  uint4 r;
-  __builtin_memcpy(&r, p, 16);
-  return r;
-}
-
 // 8 elements as they are in memory (bf16: 16 bytes, fp32: 32), zeros past K
 template <typename XT>
 struct Raw8 {
@@ -37,8 +30,8 @@ struct Raw8 {
   __device__ __forceinline__ void load(const XT* row, int c, int K) {
     constexpr bool F = std::is_same_v<XT, float>;
     if (c + 8 <= K) {
-      a = ld16(row + c);
-      if constexpr (F) b = ld16(row + c + 4);
+      a = mt::ld16(row + c);
+      if constexpr (F) b = mt::ld16(row + c + 4);
     } else {
       uint32_t w[8];
 #pragma unroll
@@ -155,7 +148,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const XT* __restrict__ 
 // them.  One wave; NV chunks of 8 columns a lane.  Returns the largest |v| as bits.
 template <int NV, typename XT>
 __device__ __forceinline__ uint32_t norm_row(const XT* xr, const float* __restrict__ gamma,
-                                             const float* __restrict__ beta, int K, float eps, bf16_t* yr, bool yvec,
+                                             const float* __restrict__ beta, int K, float eps, bf16_t* yr,
                                              int lane, float (&v)[NV][8]) {
   float sum = 0.f;
 #pragma unroll
@@ -185,9 +178,9 @@ __device__ __forceinline__ uint32_t norm_row(const XT* xr, const float* __restri
     for (int i = 0; i < 8; ++i) v[j][i] = c + i < K ? (v[j][i] - mean) * rstd * g[i] + b[i] : 0.f;
     m = max(m, umax8(v[j]));
     if (yr) {
-      if (yvec && c + 8 <= K) {
-        *reinterpret_cast<uint4*>(yr + c) = make_uint4(pack2bf(v[j][0], v[j][1]), pack2bf(v[j][2], v[j][3]),
-                                                       pack2bf(v[j][4], v[j][5]), pack2bf(v[j][6], v[j][7]));
+      if (c + 8 <= K) {
+        mt::st16(yr + c, make_uint4(pack2bf(v[j][0], v[j][1]), pack2bf(v[j][2], v[j][3]),
+                                 pack2bf(v[j][4], v[j][5]), pack2bf(v[j][6], v[j][7])));
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -202,12 +195,12 @@ template <typename XT, int NV>
 __global__ void __launch_bounds__(256) ln_quant_kernel(const XT* __restrict__ x, const float* __restrict__ gamma,
                                                        const float* __restrict__ beta, int64_t rows, int32_t K,
                                                        int64_t ldx, float eps, bf16_t* __restrict__ y, int64_t ldy,
-                                                       bool yvec, int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
+                                                       int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
   const int lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
   float v[NV][8];
-  const float s = row_scale(norm_row<NV>(x + r * ldx, gamma, beta, K, eps, y ? y + r * ldy : nullptr, yvec, lane, v));
+  const float s = row_scale(norm_row<NV>(x + r * ldx, gamma, beta, K, eps, y ? y + r * ldy : nullptr, lane, v));
   const float inv = 1.0f / s;
   int8_t* qr = q + r * ldq;
 #pragma unroll
@@ -227,29 +220,28 @@ struct LinearI8 {
   void* out;
   int64_t ldr, ldo;
   int32_t ntn, ntiles;
-  int32_t vec;   // rows of res and out are 16-byte aligned
 };
 
-// W consecutive columns of the residual's row m from n on, as they are in memory: VEC in one read, else one by one with
-// zeros past N.  RES: 0 none, 1 bf16, 2 fp32
+// W consecutive columns of the residual's row m from n on, as they are in memory: VEC in one read (at any alignment), else
+// one by one, the last column's past N.  RES: 0 none, 1 bf16, 2 fp32
 template <int W, int RES>
 struct Resid {
   uint32_t w[RES == 2 ? W : W / 2];
   template <bool VEC>
   __device__ __forceinline__ void load(const LinearI8& a, int64_t m, int n) {
     const int64_t o = m * a.ldr + n;
+    [[maybe_unused]] const int last = a.N - 1 - n;      // (may be negative: the row's last column all the same)
     if constexpr (VEC) {
-      const uint4 r = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(a.res) + o * (RES == 2 ? 4 : 2));
+      const uint4 r = mt::ld16(reinterpret_cast<const char*>(a.res) + o * (RES == 2 ? 4 : 2));
       w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
     } else if constexpr (RES == 1) {
       const bf16_t* p = reinterpret_cast<const bf16_t*>(a.res) + o;
 #pragma unroll
-      for (int c = 0; c < W; c += 2)
-        w[c / 2] = (n + c < a.N ? (uint32_t)p[c] : 0u) | (n + c + 1 < a.N ? (uint32_t)p[c + 1] << 16 : 0u);
+      for (int c = 0; c < W; c += 2) w[c / 2] = (uint32_t)p[min(c, last)] | (uint32_t)p[min(c + 1, last)] << 16;
     } else if constexpr (RES == 2) {
       const float* p = reinterpret_cast<const float*>(a.res) + o;
 #pragma unroll
-      for (int c = 0; c < W; ++c) w[c] = n + c < a.N ? __float_as_uint(p[c]) : 0u;
+      for (int c = 0; c < W; ++c) w[c] = __float_as_uint(p[min(c, last)]);
     }
   }
   __device__ __forceinline__ float get(int c) const {
@@ -274,7 +266,7 @@ __device__ __forceinline__ void finish(const LinearI8& a, int64_t m, int n, floa
   if constexpr (OUT32) {
     float* p = reinterpret_cast<float*>(a.out) + o;
     if constexpr (VEC) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+      mt::st16(p, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
     } else {
 #pragma unroll
       for (int c = 0; c < W; ++c)
@@ -283,7 +275,7 @@ __device__ __forceinline__ void finish(const LinearI8& a, int64_t m, int n, floa
   } else {
     bf16_t* p = reinterpret_cast<bf16_t*>(a.out) + o;
     if constexpr (VEC) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7]));
+      mt::st16(p, make_uint4(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])));
     } else {
 #pragma unroll
       for (int c = 0; c < W; ++c)
@@ -352,7 +344,7 @@ __device__ __forceinline__ void store_tile(const LinearI8& a, const mt::i32x4_t 
   };
   // a wave's strip of whole vectors has no branch but the one on the row (a read inside a branch is waited for there, alone:
   // 109 us instead of 86)
-  if (a.vec && n0 + wn + C::WTN <= a.N) rows(std::true_type{});
+  if (n0 + wn + C::WTN <= a.N) rows(std::true_type{});
   else rows(std::false_type{});
 }
 
@@ -387,7 +379,6 @@ struct SmallI8 {
   bf16_t* norm;
   int64_t ldn;
   float eps;
-  int32_t yvec;        // rows of norm are 16-byte aligned
   int32_t lds_ld;      // bytes of a row of q in the LDS
 };
 
@@ -399,7 +390,7 @@ __device__ __forceinline__ float small_quant(const SmallI8& a, int r, int8_t* qr
   if constexpr (NV > 0) {       // LayerNorm
     float v[NV][8];
     bf16_t* yr = a.norm && blockIdx.x == 0 ? a.norm + r * a.ldn : nullptr;
-    s = row_scale(norm_row<NV>(xr, a.gamma, a.beta, K, a.eps, yr, a.yvec, lane, v));
+    s = row_scale(norm_row<NV>(xr, a.gamma, a.beta, K, a.eps, yr, lane, v));
     const float inv = 1.0f / s;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -540,14 +531,12 @@ int quant_rows(const void* x, int64_t rows, int64_t K, int64_t ldx, int8_t* q, i
   return check_launch("dph_quant_rows_i8");
 }
 
-bool norm_vec(const DphLinearI8Args& a) { return reinterpret_cast<uintptr_t>(a.norm_out) % 16 == 0 && a.ld_norm % 8 == 0; }
-
 template <typename XT>
 int ln_quant(const DphLinearI8Args& a, hipStream_t stream) {
   with_chunks(a.K, [&](auto nv) {
     hipLaunchKernelGGL((ln_quant_kernel<XT, decltype(nv)::value>), dim3((unsigned)cdiv(a.M, 4)), dim3(256), 0, stream,
                        reinterpret_cast<const XT*>(a.x), a.ln_weight, a.ln_bias, a.M, (int32_t)a.K, a.ldx, a.ln_eps,
-                       reinterpret_cast<bf16_t*>(a.norm_out), a.ld_norm, norm_vec(a), a.q, a.ldq, a.q_scale);
+                       reinterpret_cast<bf16_t*>(a.norm_out), a.ld_norm, a.q, a.ldq, a.q_scale);
   });
   return check_launch("dph_linear_i8 (LayerNorm)");
 }
@@ -637,17 +626,15 @@ extern "C" int dph_linear_i8(const DphLinearI8Args* args, hipStream_t stream) {
     }
   }
   if (a.N == 0) return DPH_OK;
-  const int es = out32 ? 4 : 2, res = a.residual ? (out32 ? 2 : 1) : 0;
-  const uintptr_t al = reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.residual) |
-                       (uintptr_t)(a.ldo * es) | (uintptr_t)(a.residual ? a.ldr * es : 0);
+  const int res = a.residual ? (out32 ? 2 : 1) : 0;
   LinearI8 p{{reinterpret_cast<const char*>(a.q), a.ldq, (int32_t)a.M},
              {reinterpret_cast<const char*>(a.w), a.ldw, (int32_t)a.N},
              (int32_t)a.M, (int32_t)a.N, (int32_t)a.K, a.q_scale, a.w_scale, a.bias, a.residual, a.out, a.ldr, a.ldo,
-             0, 0, al % 16 == 0};
+             0, 0};
   const bool gelu = a.act == DPH_ACT_GELU;
   if (small) {
     SmallI8 sm{p, a.x, a.ldx, a.ln_weight, a.ln_bias, reinterpret_cast<bf16_t*>(a.norm_out), a.ld_norm, a.ln_eps,
-               norm_vec(a), (int32_t)small_ld(a.K)};
+               (int32_t)small_ld(a.K)};
     if (a.x_f32) launch_small<float>(sm, gelu, res, out32, stream);
     else launch_small<bf16_t>(sm, gelu, res, out32, stream);
     return check_launch("dph_linear_i8");

@@ -20,6 +20,14 @@ namespace mt {
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 
+// 16 bytes at any alignment of the element: one access, which the hardware takes
+__device__ __forceinline__ uint4 ld16(const void* p) {
+  uint4 r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+__device__ __forceinline__ void st16(void* p, uint4 r) { __builtin_memcpy(p, &r, 16); }
+
 struct I8 {
   static constexpr bool TR = false;
   typedef i32x4_t acc_t;
@@ -105,7 +113,9 @@ __device__ __forceinline__ i32x4_t keep_bytes(i32x4_t v, int nb) {
 // F16T's k-rows to a multiple of 64 (kbytes: 2 bytes a k-row).  The product is added to what init() puts into acc while
 // the first steps are on their way; it ends with a barrier, so another may follow.  S - 1 steps are in flight: with few
 // tiles a step is a load's latency unless several are.  (Seven in flight, one workgroup a CU, were slower than three: 6.2
-// against 4.9 us at 499 x 768 x 768; the next step's fragments read before this one's products changed nothing.)
+// against 4.9 us at 499 x 768 x 768; the next step's fragments read before this one's products changed nothing.  Two wave
+// groups with half of the steps each, where a CU has one tile, took 6 % off the iteration of one 768 x 768, but a result
+// would then depend on how many tiles a call has.)
 template <class T, class C, class Init>
 __device__ __forceinline__ void product(const Rows& A, const Rows& B, int32_t kbytes, int32_t m0, int32_t n0,
                                         typename T::acc_t (&acc)[C::FM][C::FN], char* smem, int wave, int lane,

@@ -85,7 +85,7 @@ __device__ __forceinline__ void add_low4q(float* v, uint32_t w, float scale) {
 struct Group {
   int32_t m, n, mp, np, cnt, wide;    // wide: the caller's matrices are m x n
   float s;                            // Y is held times s
-  int32_t vec;                        // rows of out are 16-byte aligned
+  int32_t pad;
   char *y[2], *lo, *yl[2];            // [cnt][np][mp]: fp16 x 2, then e4m3, or (split) two fp16 halves more
   char *e, *f, *el, *fl;              // [cnt][mp][mp]; the lower halves (split) or null
   double* part;                       // [cnt][NS_PARTS]
@@ -527,9 +527,9 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
         for (int r = 0; r < V::W / 2; ++r) w[r] = pack2bf(v[2 * r] * inv, v[2 * r + 1] * inv);
         bf16_t* p = g.out + (int64_t)z * rows * cols + (int64_t)m * cols + n0q;
         if (m < rows) {
-          if (g.vec && nw + C::WTN <= cols) {
+          if (nw + C::WTN <= cols) {
 #pragma unroll
-            for (int r = 0; r < V::W / 2; r += 4) *reinterpret_cast<uint4*>(p + 2 * r) = make_uint4(w[r], w[r + 1], w[r + 2], w[r + 3]);
+            for (int r = 0; r < V::W / 2; r += 4) mt::st16(p + 2 * r, make_uint4(w[r], w[r + 1], w[r + 2], w[r + 3]));
           } else {
 #pragma unroll
             for (int r = 0; r < V::W; ++r)
@@ -674,7 +674,6 @@ int run_groups(const DphNsMat* mats, const DphNsGroup* groups, int ng, int steps
     g.mp = (int32_t)up64(g.m);
     g.np = (int32_t)up64(g.n);
     g.cnt = (int32_t)in.count;
-    g.vec = in.cols % 8 == 0 && reinterpret_cast<uintptr_t>(in.out) % 16 == 0;
     g.out = reinterpret_cast<bf16_t*>(in.out);
     // entries of X0 have the mean square 1 / (m n): s is the power of two next below sqrt(m n) / 4, at most 2^14 so
     // that an entry of 1.5 times s is a finite fp16 number
