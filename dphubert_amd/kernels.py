@@ -493,7 +493,7 @@ class _on_device:
 
 def _chk_on(dev, t, name, dtypes, ndim):
     """The shape of a device tensor of these types and dimensions on ``dev``."""
-    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.device == dev and dev.type == "cuda":
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.device == dev and t.is_cuda:
         shape = t.shape
         if len(shape) == ndim:
             return shape
@@ -519,6 +519,9 @@ def _chk_rows(t, R, K, name):
 
 
 def _chk_vec(dev, t, name, n):
+    if isinstance(t, torch.Tensor) and t.dtype is F32 and t.device == dev and t.shape == (n,) and t.is_contiguous() \
+            and t.is_cuda:
+        return
     shape = _chk_on(dev, t, name, _F32_ONLY, 1)
     if shape[0] != n or not t.is_contiguous():
         raise ValueError(f"{name}: expected {n} contiguous elements, got shape {tuple(t.shape)}, strides {t.stride()}")
@@ -647,7 +650,8 @@ def _linear_i8(x, w, bias, act, residual, out, out_dtype, ln, keep_norm):
         qp, sp = x.q.data_ptr(), x.scale.data_ptr()
     else:
         xp, xf, ldq, qp, sp = x.data_ptr(), x.dtype == F32, _i8_ld(K), 0, 0
-        nbytes = M * (ldq + 4) if over else _lib.lib().dph_linear_i8_workspace(M, N, K)
+        # (above 16 rows, or where out lies over x: the integers, then the scales)
+        nbytes = M * (ldq + 4) if over or M > 16 else _lib.lib().dph_linear_i8_workspace(M, N, K)
         if nbytes:
             ws = torch.empty((nbytes,), dtype=torch.int8, device=dev)    # q, then the scales
             qp = ws.data_ptr()
