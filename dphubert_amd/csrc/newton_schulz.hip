@@ -23,7 +23,13 @@
 // Layout.  What is stored is Y = X^T ([n][m], the long side first), and only that: Y F has both operands contiguous
 // along k, and the Gram matrix reads Y through the transposing LDS read.  A step then moves Y in and out once (and its 8
 // more bits while they are held) -- with a transposed copy kept, and 16 bits more, the update of 24 matrices of 4096 x
-// 1024 wrote 600 MB and took 487 us at 850 TFLOP/s.
+// 1024 took 487 us instead of 256.
+//
+// What bounds it.  24 matrices of 1024 x 4096, a step: Gram matrix 151 us (103 GFLOP, 240 tiles: one round of CUs, half of
+// the matrix cores' cycles in use), square 45 us (26 GFLOP), product with Y 256 us (206 GFLOP and 600 MB) while the 8 bits
+// are held and 190 us after (400 MB): reading Y, products and writing take turns in a CU, whose registers hold one tile's
+// sums and nothing of the next.  (Workgroups started in a staggered order, so that some multiply while others store, gained
+// what the staggering cost.)  One matrix of 768 x 768: 17 launches of 5 to 11 us, each a chain of 12 latencies.
 #include "mfma_tile.h"
 
 #include <type_traits>
@@ -135,7 +141,7 @@ __device__ __forceinline__ int find_mat(const Mats& a, int b) {
 }
 
 // Sums of squares in 64 bits, NS_PARTS parts of a matrix, added in a fixed order later.  A matrix without gaps is read
-// as one run of 16-byte vectors, another line by line.
+// as one run of 16-byte vectors, another line by line.  Bound by memory: 403 MB in 94 us, 4.3 TB/s.
 __global__ void __launch_bounds__(256) ns_sumsq_kernel(const Mats a, const PackGroups pg) {
   const int k = find_mat(a, (int)blockIdx.x);
   const Mat& t = a.m[k];
@@ -193,7 +199,8 @@ __global__ void __launch_bounds__(256) ns_sumsq_kernel(const Mats a, const PackG
   if (threadIdx.x == 0) g.part[(int64_t)t.index * NS_PARTS + part] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// Y0, 64 x 64 tiles through the LDS; reads run along whichever stride of the input is 1
+// Y0, 64 x 64 tiles through the LDS; reads run along whichever stride of the input is 1.  Bound by memory: 403 MB read and
+// 302 written in 127 us, 5.6 TB/s.
 __global__ void __launch_bounds__(256) ns_pack_kernel(const Mats a, const PackGroups pg, float eps) {
   __shared__ float tile[64][65];
   __shared__ float scale;
@@ -316,7 +323,7 @@ __global__ void __launch_bounds__(C::NT, C::WPE) ns_product_kernel(const Groups 
   [[maybe_unused]] const int M = SYM ? g.mp : g.np, N = g.mp;      // (what lies past m and n is zero, and stays zero)
   // the sums start from 0, or from mu Y, whose rows are about to be read as an operand anyway.  All its reads are asked for
   // before the first is used, and rows past the end read the last one instead of none (a read inside a branch is waited
-  // for there: 16 latencies one after the other, 280 against 200 us for the update of 24 matrices of 4096 x 1024)
+  // for there, 32 latencies one after the other: all steps of 24 matrices of 1024 x 4096 took 2546 us instead of 2260)
   auto init = [&]() {
     if constexpr (KIND != UPDATE) {
       mt::clear<T, C>(acc);
