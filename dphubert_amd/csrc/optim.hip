@@ -142,7 +142,8 @@ __global__ void __launch_bounds__(256) adamw_kernel(const DphTensorSlot* __restr
 }
 
 // Muon: momentum and the matrix that is orthogonalised, then the step along its orthogonal factor.  Both passes are bound
-// by memory: 20 and 12 bytes a parameter (and 2 of the image).
+// by memory, 16 bytes a parameter (20 where the gradient is clipped) and 10 (12 with the image): 361 and 168 us for 24 of
+// 1024 x 4096, clipped and without images, 5.6 and 6.0 TB/s.
 __global__ void __launch_bounds__(256) muon_momentum_kernel(const DphMuonSlot* __restrict__ slots,
                                                             const int64_t* __restrict__ cslot,
                                                             const int64_t* __restrict__ cstart, Groups G,
