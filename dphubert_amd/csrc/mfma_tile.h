@@ -13,6 +13,8 @@
 #pragma once
 #include "gemm_core.h"
 
+#include <type_traits>
+
 namespace dph {
 namespace {
 namespace mt {
@@ -70,14 +72,46 @@ __device__ __forceinline__ int tr_off(int c0, int lane) {
   const int i = lane & 15, q = i >> 2, p = i & 3, k0 = 8 * (lane >> 4) + q, c = (c0 >> 3) + (p >> 1);
   return k0 * (2 * R) + ((c ^ tr_swz<R>(k0)) << 4) + ((p & 1) << 3);
 }
-template <int R>
-__device__ __forceinline__ i32x4_t tr_frag(const char* img, int off, int s) {
-  typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
-  const char* p = img + off + s * 64 * R;
-  const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-  const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * R));
-  const s16x8_t v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-  return __builtin_bit_cast(i32x4_t, v);
+// Both substeps' fragments of N column groups (c0, c0 + 16, ...), read and waited for.  Written as one block each: to the
+// compiler the builtin of this read may alias every LDS DMA in flight, and it waits for all of them before it, which leaves
+// nothing in flight across a step (the Gram matrices of 24 matrices of 1024 x 4096: 151 us with the builtin, 134 so; of one
+// of 768 x 768 11 and 8.  Two workgroups a CU hide it: 45 and 47 us for 48 of 768 x 768)
+template <int R, int N>
+__device__ __forceinline__ void tr_frags(const char* img, int c0, int lane, i32x4_t (&f)[N][2]) {
+  typedef __attribute__((ext_vector_type(2))) int i32x2_t;
+  static_assert(N == 1 || N == 2 || N == 4, "column groups of a block");
+  constexpr int O1 = 8 * R, O2 = 64 * R, O3 = 72 * R;
+  uint32_t a[N];
+  i32x2_t v[N][4];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    a[i] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)img + (uint32_t)tr_off<R>(c0 + 16 * i, lane);
+#define DPH_TR4(d0, d1, d2, d3, s)                                                                        \
+  "ds_read_b64_tr_b16 %" d0 ", %" s "\n\tds_read_b64_tr_b16 %" d1 ", %" s " offset:%c[o1]\n\t"            \
+  "ds_read_b64_tr_b16 %" d2 ", %" s " offset:%c[o2]\n\tds_read_b64_tr_b16 %" d3 ", %" s " offset:%c[o3]\n\t"
+#define DPH_TRO(i) "=&v"(v[i][0]), "=&v"(v[i][1]), "=&v"(v[i][2]), "=&v"(v[i][3])
+  if constexpr (N == 1)
+    asm volatile(DPH_TR4("0", "1", "2", "3", "4") "s_waitcnt lgkmcnt(0)"
+                 : DPH_TRO(0)
+                 : "v"(a[0]), [o1] "i"(O1), [o2] "i"(O2), [o3] "i"(O3)
+                 : "memory");
+  else if constexpr (N == 2)
+    asm volatile(DPH_TR4("0", "1", "2", "3", "8") DPH_TR4("4", "5", "6", "7", "9") "s_waitcnt lgkmcnt(0)"
+                 : DPH_TRO(0), DPH_TRO(1)
+                 : "v"(a[0]), "v"(a[1]), [o1] "i"(O1), [o2] "i"(O2), [o3] "i"(O3)
+                 : "memory");
+  else
+    asm volatile(DPH_TR4("0", "1", "2", "3", "16") DPH_TR4("4", "5", "6", "7", "17") DPH_TR4("8", "9", "10", "11", "18")
+                     DPH_TR4("12", "13", "14", "15", "19") "s_waitcnt lgkmcnt(0)"
+                 : DPH_TRO(0), DPH_TRO(1), DPH_TRO(2), DPH_TRO(3)
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), [o1] "i"(O1), [o2] "i"(O2), [o3] "i"(O3)
+                 : "memory");
+#undef DPH_TR4
+#undef DPH_TRO
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) f[i][s] = i32x4_t{v[i][2 * s][0], v[i][2 * s][1], v[i][2 * s + 1][0], v[i][2 * s + 1][1]};
 }
 
 // WR x WC waves, a ring of S steps in the LDS
@@ -179,19 +213,18 @@ __device__ __forceinline__ void product(const Rows& A, const Rows& B, int32_t kb
     // the slot that was read in the last step (every wave is past it)
     if (kt + C::S - 1 < nk) stage(kt + C::S - 1, slot == 0 ? C::S - 1 : slot - 1);
     const char* buf = smem + slot * C::BUF;
+    i32x4_t ta[C::FM][2], tb[C::FN][2];
+    if constexpr (T::TR) {
+      tr_frags<C::BM>(buf, wr * C::WTM, lane, ta);
+      tr_frags<C::BN>(buf + C::BM * 128, wc * C::WTN, lane, tb);
+    }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       i32x4_t fa[C::FM], fb[C::FN];
 #pragma unroll
-      for (int i = 0; i < C::FM; ++i) {
-        if constexpr (T::TR) fa[i] = tr_frag<C::BM>(buf, tr_off<C::BM>(wr * C::WTM + 16 * i, lane), s);
-        else fa[i] = frag(buf, wr * C::WTM + 16 * i, s, lane);
-      }
+      for (int i = 0; i < C::FM; ++i) fa[i] = T::TR ? ta[i][s] : frag(buf, wr * C::WTM + 16 * i, s, lane);
 #pragma unroll
-      for (int j = 0; j < C::FN; ++j) {
-        if constexpr (T::TR) fb[j] = tr_frag<C::BN>(buf + C::BM * 128, tr_off<C::BN>(wc * C::WTN + 16 * j, lane), s);
-        else fb[j] = frag(buf + C::BM * 128, wc * C::WTN + 16 * j, s, lane);
-      }
+      for (int j = 0; j < C::FN; ++j) fb[j] = T::TR ? tb[j][s] : frag(buf + C::BM * 128, wc * C::WTN + 16 * j, s, lane);
       if (T::ESIZE == 1 && kt * 128 + 128 > kbytes) {
         const int nb = kbytes - kt * 128 - (s * 4 + (lane >> 4)) * 16;
 #pragma unroll
@@ -315,32 +348,24 @@ __device__ __forceinline__ void product_duo(const Rows& A, const Rows& B, int32_
   };
   i32x4_t falo[C::FM2][2], fah_[C::FM2][2], fb0[C::FN0][2], fb1[C::FN1][2];
   i32x4_t(&fahi)[C::FM2][2] = C::SPLITA ? fah_ : falo;
-  auto rd_a = [&](const char* ht, i32x4_t(&fa)[C::FM2][2]) {
+  // the fragments of N groups of 16 rows from r0 on
+  auto rd = [&](const char* ht, int r0, auto& f, auto R) {
+    if constexpr (T::TR) {
+      tr_frags<decltype(R)::value>(ht, r0, lane, f);
+    } else {
+      constexpr int N = sizeof(f) / sizeof(f[0]);
 #pragma unroll
-    for (int i = 0; i < C::FM2; ++i)
+      for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if constexpr (T::TR) fa[i][s] = tr_frag<C::RA>(ht, tr_off<C::RA>(wr * HA + 16 * i, lane), s);
-        else fa[i][s] = frag(ht, wr * HA + 16 * i, s, lane);
-      }
+        for (int s = 0; s < 2; ++s) f[i][s] = frag(ht, r0 + 16 * i, s, lane);
+    }
   };
+  auto rd_a = [&](const char* ht, i32x4_t(&fa)[C::FM2][2]) { rd(ht, wr * HA, fa, std::integral_constant<int, C::RA>{}); };
   auto rd_b0 = [&](const char* bu) {
-#pragma unroll
-    for (int j = 0; j < C::FN0; ++j)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if constexpr (T::TR) fb0[j][s] = tr_frag<C::RB0>(bu + C::O_B0, tr_off<C::RB0>(wc * 16 * C::FN0 + 16 * j, lane), s);
-        else fb0[j][s] = frag(bu + C::O_B0, wc * 16 * C::FN0 + 16 * j, s, lane);
-      }
+    rd(bu + C::O_B0, wc * 16 * C::FN0, fb0, std::integral_constant<int, C::RB0>{});
   };
   auto rd_b1 = [&](const char* bu) {
-#pragma unroll
-    for (int j = 0; j < C::FN1; ++j)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if constexpr (T::TR) fb1[j][s] = tr_frag<C::RB1>(bu + C::O_B1, tr_off<C::RB1>(wc * 16 * C::FN1 + 16 * j, lane), s);
-        else fb1[j][s] = frag(bu + C::O_B1, wc * 16 * C::FN1 + 16 * j, s, lane);
-      }
+    rd(bu + C::O_B1, wc * 16 * C::FN1, fb1, std::integral_constant<int, C::RB1>{});
   };
   auto mask = [&](int u, i32x4_t(&fa)[C::FM2][2]) {
     if (!part) return;
