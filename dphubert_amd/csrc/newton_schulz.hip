@@ -23,10 +23,10 @@
 // Layout.  What is stored is Y = X^T ([n][m], the long side first), and only that: Y F has both operands contiguous
 // along k, and the Gram matrix reads Y through the transposing LDS read.  A step then moves Y in and out once (and its 8
 // more bits while they are held) -- with a transposed copy kept, and 16 bits more, the update of 24 matrices of 4096 x
-// 1024 took 487 us instead of 256.
+// 1024 took 487 us instead of 262.
 //
 // What bounds it.  24 matrices of 1024 x 4096, a step: Gram matrix 134 us (103 GFLOP, 240 tiles: one round of CUs, half of
-// the matrix cores' cycles in use), square 45 us (26 GFLOP), product with Y 256 us (206 GFLOP and 600 MB) while the 8 bits
+// the matrix cores' cycles in use), square 45 us (26 GFLOP), product with Y 262 us (206 GFLOP and 600 MB) while the 8 bits
 // are held and 190 us after (400 MB): reading Y, products and writing take turns in a CU, whose registers hold one tile's
 // sums and nothing of the next.  (Workgroups started in a staggered order, so that some multiply while others store, gained
 // what the staggering cost.)  One matrix of 768 x 768: 17 launches of 5 to 8 us, each a chain of 12 latencies.
