@@ -558,9 +558,9 @@ def _chk_out(out, x, w, bias, residual):
     """out is the residual itself, beside it (columns of one buffer), or elsewhere, and over no operand; whether it lies
     over x, which is then quantised first."""
     if residual is not None and _overlap(out, residual):
-        (ld, N), d = (out.stride(0), out.shape[1]), (out.data_ptr() - residual.data_ptr()) // out.element_size()
-        if (d or out.stride() != residual.stride()) and \
-                not (ld == residual.stride(0) and N <= d % ld <= ld - N):
+        (M, N), ld = out.shape, out.stride(0)
+        alike, d = M == 1 or ld == residual.stride(0), (out.data_ptr() - residual.data_ptr()) // out.element_size()
+        if not (alike and d == 0) and not (alike and M > 1 and N <= d % ld <= ld - N):
             raise ValueError("out overlaps the residual, but is not it")
     rows = isinstance(x, I8Rows)
     if any(t is not None and _overlap(out, t) for t in (w.q, w.scale, bias) + (tuple(x) if rows else ())):

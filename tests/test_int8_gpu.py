@@ -205,6 +205,20 @@ def test_linear_out_over_x(M, dt):
         K.linear_i8(buf[:1, :100], w, out=w.scale.view(1, 50), out_dtype=F32)
 
 
+def test_linear_one_row_in_place():
+    g = gen(17)
+    x = acts(1, 64, BF16, g)
+    w = K.quant_rows_i8(torch.randn(64, 64, generator=g).cuda())
+    want = K.linear_i8(x, w, residual=x)
+    # (a row's distance to the next one means nothing where there is none)
+    for row in (x.clone(), x.clone().as_strided((1, 64), (7, 1)), x.clone().as_strided((1, 64), (0, 1))):
+        same = row.as_strided((1, 64), (64, 1))
+        assert K.linear_i8(row, w, residual=same, out=row) is row and torch.equal(row, want)
+    buf = torch.zeros(1, 96, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        K.linear_i8(x, w, residual=buf[:, :64], out=buf[:, 32:])
+
+
 def test_gelu_of_sums_past_the_range():
     """Finite operands whose sum is infinite in fp32: GELU(inf) = inf, and GELU(-inf) has the limit 0."""
     for M in (3, 40):
