@@ -36,6 +36,8 @@ class FusedAdamW(torch.optim.Optimizer):
         self._step = 0
         self._step_t = torch.zeros((), dtype=torch.float32)   # one counter shared by every param's state
         self.dyn_ptr = None          # device DphAdamDyn (stepstate.StepScalars) -> dph_adamw_step_dev
+        self._captured = False       # a launch was captured: the graph reads the device tables by address
+        self._kept = []              # the tables that such a graph may read and that others have taken the place of
 
     def _params(self):
         out = []
@@ -44,11 +46,19 @@ class FusedAdamW(torch.optim.Optimizer):
                 out.append((gi, p))
         return out
 
+    def _replace(self, *tables):
+        """Other tables take the place of these: a graph that reads them goes on doing so."""
+        if self._captured:
+            self._kept.append(tables)
+
     def _ensure_chunks(self, plist):
-        key = tuple((p.data_ptr(), p.numel()) for _, p in plist)
+        dev = plist[0][1].device
+        key = (dev,) + tuple(p.numel() for _, p in plist)     # (moved pointers are written into the same slots)
         if key == self._chunk_key:
             return
-        dev = plist[0][1].device
+        if self._chunk_key is not None:
+            self._replace(self._cslot, self._cstart, self._slots_dev, self._sumsq)
+        self._slot_key = None
         cslot, cstart = [], []
         for si, (_, p) in enumerate(plist):
             n = p.numel()
@@ -71,6 +81,8 @@ class FusedAdamW(torch.optim.Optimizer):
     def _slot_table(self, plist):
         """Upload the (param, grad, exp_avg, exp_avg_sq) pointer table when any pointer changed.
         With a GradReducer the gradients are fixed bucket views, so this runs once."""
+        capturing = torch.cuda.is_current_stream_capturing()
+        self._captured |= capturing
         key = []
         for gi, p in plist:
             st = self.state[p]
@@ -92,7 +104,7 @@ class FusedAdamW(torch.optim.Optimizer):
         key = tuple(key)
         if key == self._slot_key:
             return
-        if torch.cuda.is_current_stream_capturing():
+        if capturing:
             raise RuntimeError("FusedAdamW: parameter/gradient storage changed inside a HIP graph capture")
         if self._event is not None:
             self._event.synchronize()     # previous H2D copy of the pinned table is done
@@ -187,8 +199,9 @@ class FusedMuon(FusedAdamW):
     with beta the group's ``momentum``.  orth(u)'s entries have the root mean square 1 / sqrt(max(rows, columns)), so a
     step has 0.2 lr, about AdamW's, and AdamW's learning rates and weight decay carry over.  The gradient norm that
     ``max_grad_norm`` clips is that of all groups.  State: ``momentum_buffer``; a parameter without a gradient is left
-    alone.  Captured in a HIP graph like FusedAdamW; the updates, their factors and the iteration's workspace are the
-    optimiser's own."""
+    alone.  Captured in a HIP graph like FusedAdamW: a replay steps with the gradients, states and images that the last
+    step outside it found (they have to live as long), and a graph captured before a group was added steps the groups it
+    knew.  The updates, their factors and the iteration's workspace are the optimiser's own."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  max_grad_norm: Optional[float] = None, momentum: float = 0.95, nesterov: bool = True,
@@ -203,7 +216,7 @@ class FusedMuon(FusedAdamW):
         self._ns = dict(steps=int(ns_steps), eps=float(ns_eps))
         if ns_coeffs is not None:
             self._ns["coeffs"] = tuple(ns_coeffs)
-        self._muon_key = self._muon_shapes = None
+        self._muon_key = self._muon_shapes = self._plan = None
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -232,7 +245,8 @@ class FusedMuon(FusedAdamW):
         return ("momentum_buffer",) if self._is_muon(gi) else super()._state_keys(gi)
 
     def _muon_tables(self, plist, dst):
-        """Slots, chunks, update buffers and the iteration's plan (rebuilt when a pointer moves)."""
+        """Slots, chunks, update buffers and the iteration's plan.  Like FusedAdamW's slots these are written in place when a
+        pointer moves, since a captured step reads them by address; other lists have their own."""
         at = [(i, gi, p) for i, (gi, p) in enumerate(plist) if self._is_muon(gi)]
         key = tuple((p.data_ptr(), p.grad.data_ptr() if p.grad is not None else 0,
                      self.state[p]["momentum_buffer"].data_ptr(), dst.get(id(p), 0), p.numel(), gi) for _, gi, p in at)
@@ -244,6 +258,8 @@ class FusedMuon(FusedAdamW):
         from . import kernels as K
         if at and shapes != self._muon_shapes:
             dev = at[0][2].device
+            if self._plan is not None:
+                self._replace(self._plan, self._m_slots, self._m_cslot, self._m_cstart, self._a_cslot, self._a_cstart)
             pad = lambda n: (n + 3) & ~3  # noqa: E731
             flat = torch.zeros(sum(pad(p.numel()) for _, _, p in at), dtype=torch.float32, device=dev)
             ups, o = [], 0
@@ -259,6 +275,7 @@ class FusedMuon(FusedAdamW):
                     for c in range(0, p.numel(), CHUNK)]
             self._a_cslot = torch.tensor([i for i, _ in rest], dtype=torch.int64, device=dev)
             self._a_cstart = torch.tensor([c for _, c in rest], dtype=torch.int64, device=dev)
+            self._m_slots = torch.empty(len(at) * _C.sizeof(DphMuonSlot), dtype=torch.uint8, device=dev)
             self._muon_shapes = shapes
         if at:
             slots = (DphMuonSlot * len(at))()
@@ -267,8 +284,7 @@ class FusedMuon(FusedAdamW):
                 s.update, s.dir = u.data_ptr(), o.data_ptr()
                 s.scale = 0.2 * math.sqrt(max(u.shape))
             # (a synchronous copy: pointers move when buffers are first laid out, not from step to step)
-            host = torch.frombuffer(bytearray(bytes(slots)), dtype=torch.uint8)
-            self._m_slots = host.to(at[0][2].device)
+            self._m_slots.copy_(torch.frombuffer(bytearray(bytes(slots)), dtype=torch.uint8))
         self._muon_key = key
 
     def _update(self, plist, dst, img, groups, clip, s):
