@@ -249,19 +249,32 @@ def f32_cat(*ts: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def i8_image(*ts: torch.Tensor) -> "K.I8Rows":
+def i8_image(*ts: torch.Tensor, again: bool = False) -> "K.I8Rows":
     """Weights (concatenated along dim 0) as 8-bit integers with one scale an output channel (kernels.quant_rows_i8),
-    cached on the first one like bf16_image (which keeps the others alive: another tensor cannot take their identity)."""
+    cached on the first one like bf16_image (which keeps the others alive: another tensor cannot take their identity).
+    again: laid out anew whatever is cached.  A captured forward reads the integers by address: those are written in place
+    when the weights change, and kept where others of another shape take their place."""
     owner = ts[0]
     key = tuple((t.device, t.data_ptr(), t._version) for t in ts)
     hit = getattr(owner, "_dph_i8", None)
-    if hit is not None and hit[0] == key and len(hit[2]) == len(ts) - 1 and all(a is b for a, b in zip(hit[2], ts[1:])):
-        return hit[1]
-    if torch.cuda.is_current_stream_capturing():
+    capturing = torch.cuda.is_current_stream_capturing()
+    if hit is not None and not again and hit.key == key and len(hit.others) == len(ts) - 1 and \
+            all(a is b for a, b in zip(hit.others, ts[1:])):
+        hit.captured |= capturing
+        return hit.rows
+    if capturing:
         raise RuntimeError("8-bit weights changed inside a HIP graph capture: run the model once before it")
-    w = ts[0].detach() if len(ts) == 1 else torch.cat([t.detach() for t in ts])
-    owner._dph_i8 = (key, K.quant_rows_i8(w), ts[1:])
-    return owner._dph_i8[1]
+    kept, captured = hit.kept if hit is not None else (), False
+    with torch.inference_mode(False), torch.no_grad():     # (so that they can be written in either mode later)
+        rows = K.quant_rows_i8(ts[0].detach() if len(ts) == 1 else torch.cat([t.detach() for t in ts]))
+        if hit is not None and hit.captured:
+            captured = hit.rows.q.shape == rows.q.shape and hit.rows.q.device == rows.q.device
+            if captured:
+                rows = K.I8Rows(*(old.copy_(new) for old, new in zip(hit.rows, rows)))
+            else:
+                kept += (hit.rows,)
+    owner._dph_i8 = types.SimpleNamespace(key=key, rows=rows, others=ts[1:], captured=captured, kept=kept)
+    return rows
 
 
 def pad8(n: int) -> int:

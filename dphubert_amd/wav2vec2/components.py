@@ -499,16 +499,12 @@ class EncoderLayer(Module):
         (a replayed training step changes weights without their versions)."""
         a, f = self.attention, self.feed_forward
         w = {}
-        if again:
-            for p in self.parameters():
-                if hasattr(p, "_dph_i8"):
-                    del p._dph_i8
         if a is not None:
-            w["qkv"] = ops.i8_image(a.q_proj.weight, a.k_proj.weight, a.v_proj.weight)
-            w["out"] = ops.i8_image(a.out_proj.weight)
+            w["qkv"] = ops.i8_image(a.q_proj.weight, a.k_proj.weight, a.v_proj.weight, again=again)
+            w["out"] = ops.i8_image(a.out_proj.weight, again=again)
         if f is not None:
-            w["up"] = ops.i8_image(f.intermediate_dense.weight)
-            w["down"] = ops.i8_image(f.output_dense.weight)
+            w["up"] = ops.i8_image(f.intermediate_dense.weight, again=again)
+            w["down"] = ops.i8_image(f.output_dense.weight, again=again)
         return w
 
     def forward(self, x: Tensor, attention_mask=None, position_bias: Optional[Tensor] = None,

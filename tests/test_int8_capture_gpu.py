@@ -1,0 +1,59 @@
+"""Captured forwards of an 8-bit encoder after its weights were laid out anew."""
+import pytest
+import torch
+
+from dphubert_amd import _lib
+from test_int8_model_gpu import _model, _wave
+
+pytestmark = pytest.mark.gpu
+
+
+def _junk():
+    """What may lie where something was freed."""
+    return [torch.full((n,), 77, dtype=torch.int8, device="cuda") for n in (1 << 10, 1 << 14, 1 << 18, 1 << 21, 1 << 22) for _ in range(6)]
+
+
+@pytest.mark.parametrize("family", ["hubert", "large"])
+def test_replay_after_quantize_int8_again(family):
+    m = _model(family, layers=1).quantize_int8()
+    w, ln = _wave()
+    layer = m.encoder.transformer.layers[0]
+    with torch.no_grad():
+        m.extract_features(w, ln)
+        held, g = w.clone(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got, _ = m.extract_features(held, ln)
+        rows = layer.int8_weights()
+        at = {k: (r.q.data_ptr(), r.scale.data_ptr()) for k, r in rows.items()}
+        for k in range(3):
+            if k == 1:          # other weights, by their version and unseen (no such image is laid out by a bf16 forward)
+                layer.attention.q_proj.weight.mul_(1.5)
+                layer.feed_forward.output_dense.weight.data.mul_(-0.5)
+            m.quantize_int8(False).quantize_int8()
+            assert at == {n: (r.q.data_ptr(), r.scale.data_ptr()) for n, r in layer.int8_weights().items()}
+            junk = _junk()
+            held.copy_(w.flip(0) if k == 2 else w)
+            g.replay()
+            eager, _ = m.extract_features(held, ln)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, eager)) and len(junk) == 30, k
+
+
+def test_trainer_goes_on_after_the_teacher_was_laid_out_again():
+    from test_graph_gpu import _batch
+    from test_muon_gpu import _trainer
+    prev = _lib.deterministic()
+    _lib.set_deterministic(True)
+    try:
+        batch = _batch()
+        one, two = _trainer(True, teacher_int8=True), _trainer(True, teacher_int8=True)
+        for step in range(6):
+            if step == 4:
+                assert two._graph is not None
+                two.module.teacher_model.quantize_int8()
+                junk = _junk()
+            a, b = one.step(batch).item(), two.step(batch).item()
+            assert a == b, step
+        assert len(junk) == 30
+    finally:
+        _lib.set_deterministic(prev)
