@@ -276,7 +276,7 @@ class FusedMuon(FusedAdamW):
             self._a_cslot = torch.tensor([i for i, _ in rest], dtype=torch.int64, device=dev)
             self._a_cstart = torch.tensor([c for _, c in rest], dtype=torch.int64, device=dev)
             self._m_slots = torch.empty(len(at) * _C.sizeof(DphMuonSlot), dtype=torch.uint8, device=dev)
-            self._muon_shapes = shapes
+        self._muon_shapes = shapes
         if at:
             slots = (DphMuonSlot * len(at))()
             for s, k, u, o, (_, _, p) in zip(slots, key, self._plan.mats, self._plan.out, at):

@@ -100,3 +100,18 @@ def test_a_group_added_later():
         _same(a, b)
         assert torch.equal(more[0], held)
     assert not torch.equal(held, more[1]) and len(junk) == 16
+
+
+def test_without_a_muon_group():
+    a, b = _params(), _params()
+    oa, ob = (FusedMuon([{"params": ps, "lr": 1e-2}], max_grad_norm=1.0) for ps in (a, b))
+    for ps, o in ((a, oa), (b, ob)):
+        _grads(ps, 1)
+        o.step()
+    graph = torch.cuda.CUDAGraph()
+    oa.begin_step()
+    with torch.cuda.graph(graph):
+        oa.launch()
+    for _ in range(3):
+        _replay(graph, ob)
+        _same(a, b)

@@ -101,3 +101,12 @@ def test_without_a_capture_nothing_is_kept():
     _update(opt)
     gc.collect()
     assert old() is None
+
+
+def test_without_a_muon_group_it_is_captured_like_adamw():
+    opt = FusedMuon([{"params": [_p(7), _p(3, 4)]}])
+    _update(opt)
+    _update(opt, capture=True)
+    opt.param_groups[0]["params"][0].grad = torch.randn(7)
+    _update(opt)
+    _update(opt, capture=True)
