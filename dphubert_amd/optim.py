@@ -250,7 +250,8 @@ class FusedMuon(FusedAdamW):
         at = [(i, gi, p) for i, (gi, p) in enumerate(plist) if self._is_muon(gi)]
         key = tuple((p.data_ptr(), p.grad.data_ptr() if p.grad is not None else 0,
                      self.state[p]["momentum_buffer"].data_ptr(), dst.get(id(p), 0), p.numel(), gi) for _, gi, p in at)
-        shapes = tuple((i, tuple(p.shape), p.device) for i, _, p in at) + (len(plist),)
+        # (the others' sizes too: their chunks are laid out here)
+        shapes = tuple((i, tuple(p.shape), p.device) for i, _, p in at) + tuple(p.numel() for _, p in plist)
         if key == self._muon_key and shapes == self._muon_shapes:
             return
         if torch.cuda.is_current_stream_capturing():

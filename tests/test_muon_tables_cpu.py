@@ -110,3 +110,12 @@ def test_without_a_muon_group_it_is_captured_like_adamw():
     opt.param_groups[0]["params"][0].grad = torch.randn(7)
     _update(opt)
     _update(opt, capture=True)
+
+
+def test_a_larger_parameter_beside_the_matrices_is_stepped_to_its_end():
+    opt = _muon()
+    _update(opt)
+    assert opt._a_cslot.tolist() == [2] and opt._a_cstart.tolist() == [0]
+    opt.param_groups[1]["params"][0] = _p(2 * optim.CHUNK + 5)
+    _update(opt)
+    assert opt._a_cslot.tolist() == [2, 2, 2] and opt._a_cstart.tolist() == [0, optim.CHUNK, 2 * optim.CHUNK]
