@@ -235,8 +235,23 @@ class FusedMuon(FusedAdamW):
         except ValueError:
             self.param_groups.pop()
             raise
-        # (the kernels' beta1; also what StepScalars uploads)
         g["betas"] = (g["momentum"], 0.0)
+
+    def _read_momentum(self):
+        """A group's momentum as it is now goes where the kernels' beta1 comes from (the uploaded scalars or the launch)."""
+        for g in self.param_groups:
+            if g.get("muon", False):
+                if not 0.0 <= g["momentum"] < 1.0:
+                    raise ValueError(f"momentum must be in [0, 1), got {g['momentum']}")
+                g["betas"] = (g["momentum"], 0.0)
+
+    def begin_step(self) -> int:
+        self._read_momentum()
+        return super().begin_step()
+
+    def launch(self):
+        self._read_momentum()
+        super().launch()
 
     def _is_muon(self, gi):
         return bool(self.param_groups[gi].get("muon", False))

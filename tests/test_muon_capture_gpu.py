@@ -115,3 +115,17 @@ def test_without_a_muon_group():
     for _ in range(3):
         _replay(graph, ob)
         _same(a, b)
+
+
+def test_momentum_that_was_changed():
+    p = torch.nn.Parameter(torch.randn(40, 30, generator=gen(2)).cuda())
+    opt = FusedMuon([{"params": [p], "lr": 1e-2, "muon": True, "momentum": 0.8}])
+    m = torch.zeros(40, 30, dtype=torch.float64)
+    for k, beta in enumerate((0.8, 0.95, 0.5)):
+        opt.param_groups[0]["momentum"] = beta
+        g = torch.randn(40, 30, generator=gen(k))
+        p.grad = g.cuda()
+        opt.step()
+        m += (g.double() - m) * (1 - beta)
+        # beta and 1 - beta in fp32, a difference, a product and a sum a step: 5 roundings of numbers up to |g| + |m| < 8
+        assert (opt.state[p]["momentum_buffer"].cpu().double() - m).abs().max() <= (k + 1) * 5 * 8 * 2.0 ** -24
