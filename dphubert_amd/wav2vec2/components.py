@@ -551,7 +551,9 @@ class EncoderLayer(Module):
                 cfg["wavlm"] = True
         a = att
         if self.int8:
-            if need or tr:
+            # (gradients of what lies before the layer are wanted of a frozen one too)
+            if need or tr or (torch.is_grad_enabled() and
+                              (x.requires_grad or (position_bias is not None and position_bias.requires_grad))):
                 raise RuntimeError("an encoder layer in 8-bit integers is forward only: eval mode without gradients "
                                    "(quantize_int8(False) goes back to bf16)")
             wl = dict(rel_tab=rel_tab, gw=gw, gb=gb, gc=gc, heads=heads) if rel_tab is not None else None
