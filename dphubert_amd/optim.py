@@ -25,8 +25,6 @@ class FusedAdamW(torch.optim.Optimizer):
                  max_grad_norm: Optional[float] = None):
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)
-        if len(self.param_groups) > 4:
-            raise ValueError("FusedAdamW supports at most 4 param groups")
         self.max_grad_norm = max_grad_norm
         self._chunk_key = None
         self._pinned = None
@@ -38,6 +36,11 @@ class FusedAdamW(torch.optim.Optimizer):
         self.dyn_ptr = None          # device DphAdamDyn (stepstate.StepScalars) -> dph_adamw_step_dev
         self._captured = False       # a launch was captured: the graph reads the device tables by address
         self._kept = []              # the tables that such a graph may read and that others have taken the place of
+
+    def add_param_group(self, group):
+        if len(self.param_groups) == 4:      # (what a DphAdamDyn holds)
+            raise ValueError(f"{type(self).__name__} supports at most 4 param groups")
+        super().add_param_group(group)
 
     def _params(self):
         out = []
