@@ -203,7 +203,8 @@ __global__ void __launch_bounds__(256) ns_sumsq_kernel(const Mats a, const PackG
 // 302 written in 127 us, 5.6 TB/s.
 __global__ void __launch_bounds__(256) ns_pack_kernel(const Mats a, const PackGroups pg, float eps) {
   __shared__ float tile[64][65];
-  __shared__ float scale;
+  __shared__ float scale;                // s / (|G| + eps) = scale 2^up: as one fp32 number it overflows for the smallest G
+  __shared__ int up;
   const int k = find_mat(a, (int)blockIdx.x);
   const Mat& t = a.m[k];
   const PackGroup& g = pg.g[t.group];
@@ -211,7 +212,11 @@ __global__ void __launch_bounds__(256) ns_pack_kernel(const Mats a, const PackGr
     double s = g.part[(int64_t)t.index * NS_PARTS + threadIdx.x];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (threadIdx.x == 0) scale = (float)((double)g.s / (sqrt(s) + (double)eps));
+    if (threadIdx.x == 0) {
+      int e;
+      scale = (float)frexp((double)g.s / (sqrt(s) + (double)eps), &e);
+      up = e;
+    }
   }
   const int b = (int)blockIdx.x - t.first, tm = g.mp >> 6;
   const int r0 = b / tm * 64, c0 = b % tm * 64;
@@ -224,10 +229,12 @@ __global__ void __launch_bounds__(256) ns_pack_kernel(const Mats a, const PackGr
   }
   __syncthreads();
   const float sc = scale;
+  const int e = up;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    if (t.ms == 1) tile[4 * i + ty][tx] = in[i] * sc;
-    else tile[tx][4 * i + ty] = in[i] * sc;
+    const float v = ldexpf(in[i], e) * sc;
+    if (t.ms == 1) tile[4 * i + ty][tx] = v;
+    else tile[tx][4 * i + ty] = v;
   }
   __syncthreads();
   const int64_t mat = (int64_t)t.index * g.np * g.mp;
