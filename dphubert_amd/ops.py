@@ -223,22 +223,34 @@ def refresh_images(updated_ids, cast_done=frozenset()) -> None:
 _CAT_REFRESH = {}   # id(concatenation) -> (owner, sources, concatenation)
 
 
-def f32_cat(*ts: torch.Tensor) -> torch.Tensor:
+def f32_cat(*ts: torch.Tensor, again: bool = False) -> torch.Tensor:
     """Concatenation of fp32 parameters (e.g. the q/k/v biases), cached like bf16_image and refreshed by
-    the optimizer's batched image refresh (one dph_copy_f32_multi launch for all of them)."""
+    the optimizer's batched image refresh (one dph_copy_f32_multi launch for all of them).  again: made anew whatever is
+    cached.  One that a captured forward reads is written in place when the parameters change, and kept where another
+    size takes its place."""
     owner = ts[0]
     key = ("f32cat",) + _version_key(ts)
     hit = getattr(owner, "_dph_cat", None)
-    if hit is not None and hit[0] == key:
+    capturing = torch.cuda.is_current_stream_capturing()
+    if hit is not None and not again and hit[0] == key:
+        if capturing:
+            hit[1]._dph_captured = True
         return hit[1]
     n = sum(t.numel() for t in ts)
-    out = torch.empty(n, dtype=F32, device=ts[0].device)
+    read = hit is not None and getattr(hit[1], "_dph_captured", False)
+    if read and not capturing and hit[1].numel() == n and hit[1].device == ts[0].device:
+        out = hit[1]
+    else:
+        out = torch.empty(n, dtype=F32, device=ts[0].device)
+        if hit is not None:
+            out._dph_kept = hit[1] if read else getattr(hit[1], "_dph_kept", None)
     rows, off = [], 0
     for t in ts:
         rows.append((t.detach().data_ptr(), out.data_ptr() + off * 4, t.numel()))
         off += t.numel()
-    if torch.cuda.is_current_stream_capturing():
+    if capturing:
         out.copy_(torch.cat([t.detach() for t in ts]))       # (tables are built outside captures)
+        out._dph_captured = True
     else:
         call("dph_copy_f32_multi", ptr(_table(rows)), len(rows), max(r[2] for r in rows), _s())
     if hit is not None:

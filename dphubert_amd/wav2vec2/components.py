@@ -496,12 +496,14 @@ class EncoderLayer(Module):
 
     def int8_weights(self, again: bool = False):
         """The layer's weights as 8-bit integers (cached per parameter version): ops.i8_image.  again: whatever is cached
-        (a replayed training step changes weights without their versions)."""
+        (a replayed training step changes weights without their versions), and the biases that go with them."""
         a, f = self.attention, self.feed_forward
         w = {}
         if a is not None:
             w["qkv"] = ops.i8_image(a.q_proj.weight, a.k_proj.weight, a.v_proj.weight, again=again)
             w["out"] = ops.i8_image(a.out_proj.weight, again=again)
+            if again:
+                ops.f32_cat(a.q_proj.bias, a.k_proj.bias, a.v_proj.bias, again=True)
         if f is not None:
             w["up"] = ops.i8_image(f.intermediate_dense.weight, again=again)
             w["down"] = ops.i8_image(f.output_dense.weight, again=again)

@@ -29,6 +29,8 @@ def test_replay_after_quantize_int8_again(family):
             if k == 1:          # other weights, by their version and unseen (no such image is laid out by a bf16 forward)
                 layer.attention.q_proj.weight.mul_(1.5)
                 layer.feed_forward.output_dense.weight.data.mul_(-0.5)
+                layer.attention.k_proj.bias.add_(0.25)
+                layer.attention.v_proj.bias.data.add_(0.5)
             m.quantize_int8(False).quantize_int8()
             assert at == {n: (r.q.data_ptr(), r.scale.data_ptr()) for n, r in layer.int8_weights().items()}
             junk = _junk()

@@ -1,4 +1,5 @@
 """The cached 8-bit weights (ops.i8_image) that a captured forward reads by address, on the host."""
+import ctypes
 import gc
 import weakref
 
@@ -100,3 +101,34 @@ def test_laid_out_in_inference_mode_and_written_outside_it():
     assert new.q is old.q
     with torch.inference_mode():
         assert ops.i8_image(*ts, again=True).q is old.q
+
+
+def test_the_biases_that_a_captured_forward_reads(monkeypatch):
+    """Their concatenation is cached beside the integers."""
+    monkeypatch.setattr(ops, "_table", lambda rows: rows)
+    monkeypatch.setattr(ops, "ptr", lambda t: t)
+    monkeypatch.setattr(ops, "_s", lambda: 0)
+    copy = lambda name, rows, n, most, s: [ctypes.memmove(to, at, 4 * k) for at, to, k in rows]  # noqa: E731
+    monkeypatch.setattr(ops, "call", copy)
+    ts = [torch.nn.Parameter(torch.randn(4), requires_grad=False) for _ in range(3)]
+    free, want = ops.f32_cat(*ts), torch.cat(ts)
+    assert torch.equal(free, want) and ops.f32_cat(*ts) is free
+    ts[1].mul_(2)
+    old = ops.f32_cat(*ts)
+    assert old is not free and torch.equal(free, want)        # (no graph reads it: left to its holder)
+    CAPTURING[0] = True
+    assert ops.f32_cat(*ts) is old
+    CAPTURING[0] = False
+    ts[2].mul_(3)
+    assert ops.f32_cat(*ts) is old and torch.equal(old, torch.cat(ts))
+    ts[0].data.mul_(5)                                        # (unseen)
+    assert not torch.equal(ops.f32_cat(*ts), torch.cat(ts))
+    assert ops.f32_cat(*ts, again=True) is old and torch.equal(old, torch.cat(ts))
+    at = weakref.ref(old)
+    del old
+    for n in (6, 5):
+        ts[0].data = torch.randn(n)
+        ts[1].mul_(2)
+        assert ops.f32_cat(*ts).numel() == n + 8
+        gc.collect()
+        assert at() is not None
