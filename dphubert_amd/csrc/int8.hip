@@ -370,7 +370,7 @@ __device__ __forceinline__ void store_tile(const LinearI8& a, const mt::i32x4_t 
 }
 
 // The tiles of mfma_tile.h with the scales, the activation and the residual in the epilogue.  8192 x 8192 x 8192 398 us (2760
-// TOP/s); 7984 x 1024 x 4096 36 us (1860 TOP/s), with an fp32 residual 41; 7984 x 4096 x 1024 39 us, with GELU 51, with an
+// TOP/s; 455 us on a device that clocks lower); 7984 x 1024 x 4096 36 us (1860 TOP/s), with an fp32 residual 41; 7984 x 4096 x 1024 39 us, with GELU 51, with an
 // fp32 residual 84 (262 MB).  Long sums are bound by the passage of operands through the LDS; short ones by the epilogue,
 // 14 instructions an element for GELU or memory, which a CU's one workgroup does not overlap with products, and two
 // workgroups, whose smaller tiles move more through the LDS, overlap in part.
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(C::NT, C::WPE) linear_i8_kernel(const LinearI8
 // Up to 16 rows of x in one launch: a workgroup quantises all of them for itself (they come from the L2), into the LDS,
 // and multiplies 16 channels of W, read once and straight into the registers, a quarter of K a wave.  What bounds it is
 // the latency of one read of x, the quantiser's reductions and one read of W, asked for before them: 4.1 us for one row of
-// 1024 and 4096 channels (W's 4.2 MB at a copy's rate: 0.9 us).
+// 1024 and 4096 channels in a replayed graph, 4.9 by the kernel trace (W's 4.2 MB at a copy's rate: 0.9 us).
 struct SmallI8 {
   LinearI8 l;
   const void* x;

@@ -25,9 +25,9 @@
 // more bits while they are held) -- with a transposed copy kept, and 16 bits more, the update of 24 matrices of 4096 x
 // 1024 took 487 us instead of 262.
 //
-// What bounds it.  24 matrices of 1024 x 4096, a step: Gram matrix 134 us (103 GFLOP, 240 tiles: one round of CUs, half of
-// the matrix cores' cycles in use), square 45 us (26 GFLOP), product with Y 262 us (206 GFLOP and 600 MB) while the 8 bits
-// are held and 190 us after (400 MB): reading Y, products and writing take turns in a CU, whose registers hold one tile's
+// What bounds it.  24 matrices of 1024 x 4096, a step: Gram matrix 133 us (103 GFLOP, 240 tiles: one round of CUs, 55 % of
+// the matrix cores' cycles in use), square 45 us (26 GFLOP), product with Y 254 us (206 GFLOP and 600 MB) while the 8 bits
+// are held and 191 us after (400 MB): reading Y, products and writing take turns in a CU, whose registers hold one tile's
 // sums and nothing of the next.  (Workgroups started in a staggered order, so that some multiply while others store, gained
 // what the staggering cost.)  One matrix of 768 x 768: 17 launches of 5 to 8 us, each a chain of 12 latencies.
 #include "mfma_tile.h"
@@ -141,7 +141,7 @@ __device__ __forceinline__ int find_mat(const Mats& a, int b) {
 }
 
 // Sums of squares in 64 bits, NS_PARTS parts of a matrix, added in a fixed order later.  A matrix without gaps is read
-// as one run of 16-byte vectors, another line by line.  Bound by memory: 403 MB in 94 us, 4.3 TB/s.
+// as one run of 16-byte vectors, another line by line.  Bound by memory: 403 MB in 93 us, 4.3 TB/s.
 __global__ void __launch_bounds__(256) ns_sumsq_kernel(const Mats a, const PackGroups pg) {
   const int k = find_mat(a, (int)blockIdx.x);
   const Mat& t = a.m[k];
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256) ns_sumsq_kernel(const Mats a, const PackG
 }
 
 // Y0, 64 x 64 tiles through the LDS; reads run along whichever stride of the input is 1.  Bound by memory: 403 MB read and
-// 302 written in 127 us, 5.6 TB/s.
+// 302 written in 123 us, 5.7 TB/s.
 __global__ void __launch_bounds__(256) ns_pack_kernel(const Mats a, const PackGroups pg, float eps) {
   __shared__ float tile[64][65];
   __shared__ float scale;                // s / (|G| + eps) = scale 2^up: as one fp32 number it overflows for the smallest G

@@ -768,7 +768,8 @@ class NewtonSchulzPlan:
 def newton_schulz(mats: Sequence[torch.Tensor], *, steps: int = 5, coeffs: Sequence[float] = NS_COEFFS,
                   eps: float = 1e-7) -> List[torch.Tensor]:
     """The orthogonal factor of every matrix of the list, approximately: ``steps`` quintic Newton-Schulz steps
-    X <- a X + (b A + c A^2) X, A = X X^T, from X = G / (|G|_F + eps) (of G^T where G is taller than wide).
+    X <- a X + (b A + c A^2) X, A = X X^T, from X = G / (|G|_F + eps) (of G^T where G is taller than wide).  The default
+    coefficients are those published with Muon (Jordan et al., 2024).
 
     mats: 2-D tensors of one device, bf16 or fp32, of any shapes and row strides (a transposed view will do).  Returns
     bf16 tensors of the same shapes.  Matrices of all shapes share launches, so hand in a whole model's at once.  The

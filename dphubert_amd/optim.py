@@ -200,7 +200,8 @@ class FusedMuon(FusedAdamW):
         p <- p (1 - lr weight_decay) - lr 0.2 sqrt(max(rows, columns)) orth(u)
 
     with beta the group's ``momentum``.  orth(u)'s entries have the root mean square 1 / sqrt(max(rows, columns)), so a
-    step has 0.2 lr, about AdamW's, and AdamW's learning rates and weight decay carry over.  The gradient norm that
+    step has 0.2 lr, about AdamW's, and AdamW's learning rates and weight decay carry over (Jordan et al., 2024; the factor
+    0.2 sqrt(max) and the decay: Liu et al., 2025).  A group's ``momentum`` may change between steps.  The gradient norm that
     ``max_grad_norm`` clips is that of all groups.  State: ``momentum_buffer``; a parameter without a gradient is left
     alone.  Captured in a HIP graph like FusedAdamW: a replay steps with the gradients, states and images that the last
     step outside it found (they have to live as long), and a graph captured before a group was added steps the groups it

@@ -134,7 +134,8 @@ class Wav2Vec2Model(Module):
         """Run the encoder layers' projections (query / key / value, output, both feed-forward ones) in 8-bit integers:
         weights with one scale an output channel, laid out now and again whenever they change, activations with one
         scale a token.  Forward only -- eval mode, no gradients: a frozen teacher, inference of a pruned student.  The
-        rest of the model, and the hidden states' types, stay as they are.  ``enable=False`` goes back to bf16."""
+        rest of the model, and the hidden states' types, stay as they are.  A captured forward goes on with what a later
+        call lays out (in the same memory).  ``enable=False`` goes back to bf16."""
         layers = self.encoder.transformer.layers
         if enable:
             for layer in layers:
