@@ -59,6 +59,8 @@ class FusedAdamW(torch.optim.Optimizer):
         key = (dev,) + tuple(p.numel() for _, p in plist)     # (moved pointers are written into the same slots)
         if key == self._chunk_key:
             return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{type(self).__name__}: the parameter list changed inside a HIP graph capture")
         if self._chunk_key is not None:
             self._replace(self._cslot, self._cstart, self._slots_dev, self._sumsq)
         self._slot_key = None

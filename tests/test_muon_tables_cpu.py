@@ -119,3 +119,16 @@ def test_a_larger_parameter_beside_the_matrices_is_stepped_to_its_end():
     opt.param_groups[1]["params"][0] = _p(2 * optim.CHUNK + 5)
     _update(opt)
     assert opt._a_cslot.tolist() == [2, 2, 2] and opt._a_cstart.tolist() == [0, optim.CHUNK, 2 * optim.CHUNK]
+
+
+def test_a_capture_that_would_need_other_tables_is_refused_and_leaves_them():
+    opt = _muon()
+    _update(opt)
+    old = [getattr(opt, n) for n in ("_slots_dev", "_cslot", "_m_slots", "_plan")]
+    opt.add_param_group({"params": [_p(6, 6)]})
+    with pytest.raises(RuntimeError, match="capture"):
+        _update(opt, capture=True)
+    CAPTURING[0] = False
+    assert all(getattr(opt, n) is t for n, t in zip(("_slots_dev", "_cslot", "_m_slots", "_plan"), old))
+    _update(opt)
+    assert opt._cslot.tolist() == [0, 1, 2, 3]
